@@ -41,7 +41,7 @@ def main():
     else:
       with tempfile.TemporaryDirectory() as tmp:
         asm = os.path.join(tmp, "gemm_bx.s")
-        subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
+        subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                         "-I", os.path.join(ROOT, "include"), "-I", os.path.dirname(SRC), "-S", "--cuda-device-only", SRC,
                         "-o", asm], check=True, stderr=subprocess.DEVNULL)
         text = open(asm).read()

@@ -13,7 +13,7 @@ CSRC = os.path.join(ROOT, "pytorch_geometric_temporal_amd", "csrc")
 def main():
     src = os.path.join(CSRC, sys.argv[1])
     pat = sys.argv[2] if len(sys.argv) > 2 else ""
-    out = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
+    out = subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                           "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-c", src, "-o", "/dev/null",
                           "-Rpass-analysis=kernel-resource-usage"], capture_output=True, text=True).stderr
     cur = None
