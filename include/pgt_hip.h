@@ -51,7 +51,7 @@ extern "C" {
 #define PGT_ERR_LAUNCH (-2)    /* HIP reported an error at launch */
 #define PGT_ERR_WORKSPACE (-3) /* scratch buffer too small */
 
-#define PGT_ABI_VERSION 17
+#define PGT_ABI_VERSION 18
 
 typedef void* pgt_stream_t; /* hipStream_t */
 
@@ -713,6 +713,46 @@ int pgt_adam_f32(float* p, const float* g, float* m, float* v, float* step, int6
  * (out-of-range rows are clamped, never read outside the series). */
 int pgt_window_gather_f32(const float* data, int64_t T_total, int64_t W, const int64_t* idx, int64_t B, int64_t h,
                           float* X, float* Y, int time_major, pgt_stream_t stream);
+
+/* Gated delta rule (csrc/delta_*.hip): a recurrent layer's memory, per sequence (sample, node, head) a state S [key, value]:
+ *   S_t = exp(g_t) S_{t-1} + k_t u_t^T,  u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t),  o_t = scale S_t^T q_t.
+ * q, k [batch, step, node, k_heads, key] and v [batch, step, node, heads, value] in one of three types, g and beta
+ * [batch, step, node, heads] in fp32, all through pgt_seq_view: element strides of the leading four axes, unit stride along the last (g,
+ * beta: none).  Value head h reads key head h / (heads / k_heads).  States, gradients of g / beta and everything inside are fp32.
+ * lengths [batch, node] (NULL: all `steps`; values outside 0 .. steps are clamped): steps from lengths on leave the state as it is,
+ * their outputs and gradients are 0 and their inputs are not looked at.  g = -inf forgets the state.  key, value: 1 .. 128.
+ * pgt_gated_delta_segments: > 1 where a sequence is walked in that many segments side by side (few sequences, many steps); the
+ * caller then brings seg_start [sequences, segments - 1, key, value] and seg_trans [sequences, segments - 2, key, key] (and keeps seg_trans
+ * for the adjoint), sequence = (sample * nodes + node) * heads + head.  Negative: an error code.
+ * Forward: start (NULL: 0) and last [sequences, key, value]; o [batch, steps, node, heads, value] contiguous.  e [as o, fp32] and states
+ * [sequences, ceil(steps / 16) - 1, key, value] are kept for the adjoint (NULL: no adjoint follows).
+ * Adjoint: d_o like o, contiguous; d_last NULL: 0; d_start NULL: not wanted.  dq, dk [batch, steps, node, k_heads, key], dv, in the
+ * inputs' type, contiguous; dg, dbeta [batch, steps, node, heads].  head_ws (heads > k_heads): 2 sequences * steps * key floats.
+ * seg_end (segments > 1): like seg_start.  Sums run in a fixed order: results do not change from call to call.
+ * Step: steps = 1, views without a step axis, state [sequences, key, value] updated in place, o [sequences, value]. */
+#define PGT_DT_F32 0
+#define PGT_DT_BF16 1
+#define PGT_DT_F16 2
+typedef struct pgt_delta_dims {
+  int64_t batch, steps, nodes;
+  int32_t k_heads, heads, key, value, dtype;
+  float scale;
+  const int32_t* lengths;
+} pgt_delta_dims;
+typedef struct pgt_seq_view {
+  const void* data;
+  int64_t batch, step, node, head;
+} pgt_seq_view;
+int pgt_gated_delta_segments(const pgt_delta_dims* dims);
+int pgt_gated_delta_fwd(const pgt_delta_dims* dims, const pgt_seq_view* q, const pgt_seq_view* k, const pgt_seq_view* v,
+                        const pgt_seq_view* g, const pgt_seq_view* beta, const float* start, void* o, float* last, float* e,
+                        float* states, float* seg_start, float* seg_trans, pgt_stream_t stream);
+int pgt_gated_delta_bwd(const pgt_delta_dims* dims, const pgt_seq_view* q, const pgt_seq_view* k, const pgt_seq_view* g,
+                        const pgt_seq_view* beta, const float* start, const float* e, const float* states, const float* seg_trans,
+                        const void* d_o, const float* d_last, void* dq, void* dk, void* dv, float* dg, float* dbeta, float* d_start,
+                        float* head_ws, float* seg_end, pgt_stream_t stream);
+int pgt_gated_delta_step(const pgt_delta_dims* dims, const pgt_seq_view* q, const pgt_seq_view* k, const pgt_seq_view* v,
+                         const pgt_seq_view* g, const pgt_seq_view* beta, float* state, void* o, pgt_stream_t stream);
 
 #ifdef __cplusplus
 }

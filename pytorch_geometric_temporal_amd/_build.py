@@ -13,7 +13,9 @@ LIB_PATH = os.path.join(LIB_DIR, "libpgt_hip.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 SOURCES = ["pgt_core.hip", "spmm.hip", "dconv_slab.hip", "gemm.hip", "gemm_bx.hip", "elementwise.hip",
-           "graph_prep.hip", "attention.hip", "evolve.hip", "small_cell.hip", "small_gcn.hip", "tconv.hip", "tgcn.hip", "seq_small.hip", "tgcn_cell.hip", "tile_order.hip", "readout.hip", "seq64.hip"]
+           "graph_prep.hip", "attention.hip", "evolve.hip", "small_cell.hip", "small_gcn.hip", "tconv.hip", "tgcn.hip", "seq_small.hip", "tgcn_cell.hip", "tile_order.hip", "readout.hip", "seq64.hip",
+           "delta_fwd.hip", "delta_bwd.hip", "delta_step.hip"]
+HEADERS = ["pgt_common.h", "delta_common.h"]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  The compiler makes them from ordinary float code, and some of their forms have
 # given wrong results on MI355X now and then.  (The host pass warns that it does not know the feature.)
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-munsafe-fp-atomics",
@@ -34,8 +36,7 @@ def source_digest():
     old kernels)."""
     import hashlib
     h = hashlib.sha256()
-    for f in [os.path.join(CSRC, s) for s in SOURCES] + [os.path.join(CSRC, "pgt_common.h"),
-                                                       os.path.join(INCLUDE, "pgt_hip.h")]:
+    for f in [os.path.join(CSRC, s) for s in SOURCES + HEADERS] + [os.path.join(INCLUDE, "pgt_hip.h")]:
         with open(f, "rb") as fh:
             h.update(fh.read())
     return h.hexdigest()
@@ -57,7 +58,7 @@ def build_hip_library(force=False, verbose=False):
     os.makedirs(LIB_DIR, exist_ok=True)
     obj_dir = os.path.join(LIB_DIR, "obj")
     os.makedirs(obj_dir, exist_ok=True)
-    headers = [os.path.join(CSRC, "pgt_common.h"), os.path.join(INCLUDE, "pgt_hip.h"), os.path.abspath(__file__)]   # (the flags stand here)
+    headers = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.join(INCLUDE, "pgt_hip.h"), os.path.abspath(__file__)]   # (the flags stand here)
     objs, relink, jobs = [], force, []
     for src in SOURCES:
         s = os.path.join(CSRC, src)

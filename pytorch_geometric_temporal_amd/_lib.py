@@ -53,6 +53,21 @@ class RowMapStruct(ctypes.Structure):
     _fields_ = [("period", c_i64), ("stride_hi", c_i64)]
 
 
+class DeltaDimsStruct(ctypes.Structure):
+    """pgt_delta_dims"""
+    _fields_ = [("batch", c_i64), ("steps", c_i64), ("nodes", c_i64), ("k_heads", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("key", ctypes.c_int32), ("value", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", c_f32), ("lengths", c_ptr)]
+
+
+class SeqViewStruct(ctypes.Structure):
+    """pgt_seq_view: element strides of [batch, step, node, head]."""
+    _fields_ = [("data", c_ptr), ("batch", c_i64), ("step", c_i64), ("node", c_i64), ("head", c_i64)]
+
+
+c_dims = ctypes.POINTER(DeltaDimsStruct)
+c_view = ctypes.POINTER(SeqViewStruct)
+
+
 class SymGraphStruct(ctypes.Structure):
     _fields_ = [("fwd", CsrStruct), ("bwd", CsrStruct), ("deg", c_ptr), ("info", c_ptr)]
 
@@ -190,9 +205,15 @@ PROTOTYPES = {
                                       c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr]),
     "pgt_tgcn_cell_bwd_acc_f32": (c_int, [c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64,
                                           c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_i64, c_ptr]),
+    "pgt_gated_delta_segments": (c_int, [c_dims]),
+    "pgt_gated_delta_fwd": (c_int, [c_dims, c_view, c_view, c_view, c_view, c_view, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
+                                    c_ptr]),
+    "pgt_gated_delta_bwd": (c_int, [c_dims, c_view, c_view, c_view, c_view, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
+                                    c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
+    "pgt_gated_delta_step": (c_int, [c_dims, c_view, c_view, c_view, c_view, c_view, c_ptr, c_ptr, c_ptr]),
 }
 
-EXPECTED_ABI = 17
+EXPECTED_ABI = 18
 
 
 class PgtLib:

@@ -1,0 +1,218 @@
+// Shared by the gated delta rule's kernels (delta_fwd.hip, delta_bwd.hip, delta_step.hip) and by group_norm.hip: storage types,
+// row-of-sixteen lane moves, the 16 x 16 tile algebra.
+//
+// The rule, per head, with state S [K, V], log decay g <= 0, write strength beta, query q, key k, value v:
+//   S_t = exp(g_t) S_{t-1} + k_t u_t^T,   u_t = beta_t e_t,   e_t = v_t - exp(g_t) S_{t-1}^T k_t,   o_t = scale S_t^T q_t.
+// Over a chunk of C = 16 steps with start state S0, c_i = g_1 + .. + g_i, D_ij = exp(c_i - c_j), Gamma = diag(exp(c_i)):
+//   (I + A') E = Y,  Y = V - Gamma K S0,  A'_ij = D_ij (k_i . k_j) beta_j  (j < i);      U = diag(beta) E
+//   O = Gamma Q S0 + P U,  P_ij = D_ij (q_i . k_j)  (j <= i);      S1 = exp(c_C) S0 + sum_j exp(c_C - c_j) k_j u_j^T.
+// C = 16 is one MFMA tile: A' and P are one tile each, (I + A')^-1 is solved in the registers of a row of sixteen lanes, and the
+// state lives in accumulator registers, where v_mfma_f32_16x16x4_f32's result layout (lane: column l % 16, rows 4 (l / 16) + r)
+// IS its B-operand layout for the contraction order k = 16 t + 4 (l / 16) + r: the state feeds the next product without a move.
+#pragma once
+#include "pgt_common.h"
+
+namespace gd {
+
+struct bf16 { uint16_t u; };
+struct f16 { uint16_t u; };
+
+#ifdef PGT_EMU
+#include "pgt_gd_platform_emu.h"
+#else
+typedef float gd_f4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ gd_f4 gd_mfma(float a, float b, gd_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// value of lane J of the row of sixteen (DPP row_newbcast)
+template <int J> __device__ __forceinline__ float gd_bcast16(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + J, 0xf, 0xf, true));
+}
+template <int N> __device__ __forceinline__ float gd_ror16(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + N, 0xf, 0xf, true));
+}
+template <int N> __device__ __forceinline__ double gd_shr16(double x) {      // lane i takes lane i - N of its row, 0 where there is none
+  const uint64_t b = __double_as_longlong(x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, 0x110 + N, 0xf, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), 0x110 + N, 0xf, 0xf, true);
+  return __longlong_as_double(((uint64_t)hi << 32) | lo);
+}
+// LDS hand-off inside one wavefront / inside the workgroup (global loads and stores stay in flight across it)
+__device__ __forceinline__ void gd_wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void gd_block_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ float gd_as_float(uint32_t u) { return __uint_as_float(u); }
+__device__ __forceinline__ uint16_t gd_to_bf16(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+__device__ __forceinline__ float gd_from_f16(uint16_t h) { return (float)__builtin_bit_cast(_Float16, h); }
+__device__ __forceinline__ uint16_t gd_to_f16(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+#endif
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(bf16 x) { return gd_as_float((uint32_t)x.u << 16); }
+__device__ __forceinline__ float to_f32(f16 x) { return gd_from_f16(x.u); }
+template <class IO> __device__ __forceinline__ IO from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ bf16 from_f32<bf16>(float x) { return bf16{gd_to_bf16(x)}; }
+template <> __device__ __forceinline__ f16 from_f32<f16>(float x) { return f16{gd_to_f16(x)}; }
+
+// four values of a row from p on, of which the first n exist (the others are 0); vec: p is aligned to four values and n is 4 or <= 0
+__device__ __forceinline__ gd_f4 load4(const float* p, int n, bool vec) {
+  gd_f4 r;
+  r[0] = r[1] = r[2] = r[3] = 0.f;
+  if (vec) {
+    if (n >= 4) { const float4 t = *reinterpret_cast<const float4*>(p); r[0] = t.x; r[1] = t.y; r[2] = t.z; r[3] = t.w; }
+    return r;
+  }
+  if (n > 0) r[0] = p[0];
+  if (n > 1) r[1] = p[1];
+  if (n > 2) r[2] = p[2];
+  if (n > 3) r[3] = p[3];
+  return r;
+}
+template <class IO> __device__ __forceinline__ gd_f4 load4(const IO* p, int n, bool vec) {
+  gd_f4 r;
+  r[0] = r[1] = r[2] = r[3] = 0.f;
+  if (vec) {
+    if (n >= 4) {
+      const int2 t = *reinterpret_cast<const int2*>(p);
+      r[0] = to_f32(IO{(uint16_t)((uint32_t)t.x & 0xffffu)}); r[1] = to_f32(IO{(uint16_t)((uint32_t)t.x >> 16)});
+      r[2] = to_f32(IO{(uint16_t)((uint32_t)t.y & 0xffffu)}); r[3] = to_f32(IO{(uint16_t)((uint32_t)t.y >> 16)});
+    }
+    return r;
+  }
+  if (n > 0) r[0] = to_f32(p[0]);
+  if (n > 1) r[1] = to_f32(p[1]);
+  if (n > 2) r[2] = to_f32(p[2]);
+  if (n > 3) r[3] = to_f32(p[3]);
+  return r;
+}
+__device__ __forceinline__ gd_f4 zero4() { gd_f4 r; r[0] = r[1] = r[2] = r[3] = 0.f; return r; }
+__device__ __forceinline__ gd_f4 lds4(const float* p) {
+  const float4 t = *reinterpret_cast<const float4*>(p);
+  gd_f4 r;
+  r[0] = t.x; r[1] = t.y; r[2] = t.z; r[3] = t.w;
+  return r;
+}
+__device__ __forceinline__ void put4(float* p, gd_f4 x) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
+// c += A B over sixteen contraction steps, k = 4 (l / 16) + r
+__device__ __forceinline__ gd_f4 mma16(gd_f4 a, gd_f4 b, gd_f4 c) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) c = gd_mfma(a[r], b[r], c);
+  return c;
+}
+__device__ __forceinline__ float sum16(float x) {       // the sum over the row of sixteen lanes, in every one of them
+  x += gd_ror16<8>(x);
+  x += gd_ror16<4>(x);
+  x += gd_ror16<2>(x);
+  x += gd_ror16<1>(x);
+  return x;
+}
+// X = (I + A)^-1 for A strictly lower triangular, lane l holding row i = l % 16 of A in a[] and X[i][4 (l / 16) + c] in t[c] (at first the
+// unit matrix).  Forward substitution, one broadcast row a step: backward stable, no powers of A.  a[j] is 0 for j >= i.
+template <int J> __device__ __forceinline__ void solve_down(const float (&a)[16], gd_f4& t) {
+  if constexpr (J < 15) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) t[c] = fmaf(-a[J], gd_bcast16<J>(t[c]), t[c]);
+    solve_down<J + 1>(a, t);
+  }
+}
+// the same for A strictly upper triangular, from the last row up; a[j] is 0 for j <= i
+template <int J> __device__ __forceinline__ void solve_up(const float (&a)[16], gd_f4& t) {
+  if constexpr (J > 0) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) t[c] = fmaf(-a[J], gd_bcast16<J>(t[c]), t[c]);
+    solve_up<J - 1>(a, t);
+  }
+}
+__device__ __forceinline__ gd_f4 unit_row(int lane) {
+  gd_f4 t;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) t[c] = ((lane & 15) == 4 * (lane >> 4) + c) ? 1.f : 0.f;
+  return t;
+}
+__device__ __forceinline__ void row16(const float* p, float (&a)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const gd_f4 x = lds4(p + 4 * q);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) a[4 * q + c] = x[c];
+  }
+}
+
+// ---- decays of a chunk.  Lane i of each row of sixteen brings g_i (0 behind the sequence) and takes the running sum c_i as a pair of
+// floats: c_i - c_j is then exact to a rounding of the DIFFERENCE, also behind a step that resets the state (g = -inf counts as
+// -200, whose exponential is 0 in fp32: differences across it vanish, differences behind it do not feel it).
+struct Decay { float hi, lo, enter, leave, whole; };
+__device__ __forceinline__ Decay chunk_decay(float g) {
+  if (g < -200.f) g = -200.f;                             // (a nan stays)
+  double c = (double)g;
+  c += gd_shr16<1>(c);
+  c += gd_shr16<2>(c);
+  c += gd_shr16<4>(c);
+  c += gd_shr16<8>(c);
+  Decay d;
+  d.hi = (float)c;
+  d.lo = (float)(c - (double)d.hi);
+  const float lh = gd_bcast16<15>(d.hi), ll = gd_bcast16<15>(d.lo);
+  d.enter = expf(d.hi + d.lo);
+  d.leave = expf((lh - d.hi) + (ll - d.lo));
+  d.whole = gd_bcast16<15>(d.enter);
+  return d;
+}
+
+constexpr int TS = 20;           // row stride of a 16 x 16 tile in LDS: the four row groups of a result tile land in different banks
+constexpr int TILE = 16 * TS;
+
+struct View { const void* p; int64_t sb, st, sn, sh; };
+
+// ---- one sequence (sample b, node n, head h) of a launch, p = (b N + n) H + h
+struct Shape {
+  int64_t P, p0;                 // sequences, first sequence of this launch
+  int N, H, rep, T, K, V, chunks, cps, segs;
+  const int32_t* lengths;        // [B, N] or null
+  float scale;
+};
+struct Seq { int64_t p; int64_t bn; int b, n, h, len; bool live; };
+__device__ __forceinline__ Seq seq_of(const Shape& s, int64_t p) {
+  Seq q;
+  q.live = p < s.P;
+  q.p = q.live ? p : 0;
+  q.bn = q.p / s.H;
+  q.h = (int)(q.p - q.bn * s.H);
+  q.b = (int)(q.bn / s.N);
+  q.n = (int)(q.bn - (int64_t)q.b * s.N);
+  int len = s.T;
+  if (s.lengths) { len = s.lengths[q.bn]; len = len < 0 ? 0 : len > s.T ? s.T : len; }
+  q.len = q.live ? len : 0;
+  return q;
+}
+template <class T> __device__ __forceinline__ const T* at(const View& v, const Seq& q, int h) {
+  return reinterpret_cast<const T*>(v.p) + (int64_t)q.b * v.sb + (int64_t)q.n * v.sn + (int64_t)h * v.sh;
+}
+// chunks that any of the workgroup's sequences reaches (the same in every thread)
+template <int TEAMS> __device__ __forceinline__ int chunks_of_block(const Shape& s, int64_t first) {
+  int most = 0;
+#pragma unroll
+  for (int i = 0; i < TEAMS; ++i) {
+    const int len = seq_of(s, first + i).len;
+    most = len > most ? len : most;
+  }
+  return (most + 15) / 16;
+}
+
+template <int D> struct Team {             // a team of wavefronts owns a sequence: one wavefront to 16 columns of the padded width
+  static constexpr int NW = D / 16;
+  static constexpr int TEAMS = NW >= 4 ? 1 : 4 / NW;
+  static constexpr int TL = 64 * NW;
+  static constexpr int THREADS = TL * TEAMS;
+  static constexpr int LD = D + 4;         // LDS row stride: rows of sixteen lanes x 16 bytes cover the banks once
+  static constexpr int EPL = TL >= 256 ? 1 : 256 / TL;      // elements of a 16 x 16 tile a lane
+};
+template <int D> __device__ __forceinline__ void team_sync() {
+  if constexpr (Team<D>::NW == 1) gd_wave_sync(); else gd_block_sync();
+}
+
+}  // namespace gd
+
+// host side (delta_fwd.hip): the checked shape with its plan, views, whether rows can be read four values at a time, the adjoint's join
+int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s);
+gd::View pgt_delta_view(const pgt_seq_view* v);
+bool pgt_delta_vec(const pgt_seq_view* v, int width, int dtype);
+int pgt_delta_join_up(const float* trans, float* x, int64_t P, int segs, int K, int V, pgt_stream_t stream);

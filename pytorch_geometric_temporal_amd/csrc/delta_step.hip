@@ -1,0 +1,172 @@
+// Gated delta rule, one step of every sequence, the state updated in place (delta_common.h has the rule):
+//   held = exp(g) S^T k,  u = beta (v - held),  S <- exp(g) S + k u^T,  o = scale S^T q = scale (exp(g) S_old^T q + (q . k) u).
+// The second form of o takes both products from ONE pass over the old state, which then waits in registers for its update: the
+// state crosses HBM once each way and nothing else is of size.  Bound by that traffic (8 K V bytes a sequence).
+#include "delta_common.h"
+
+using namespace gd;
+
+namespace {
+
+struct StepArgs {
+  int64_t P, p0;
+  int N, H, rep, K, V;
+  float scale;
+  View q, k, v, g, beta;          // (step strides unused)
+  float* state;                   // [P, K, V]
+  void* o;                        // [P, V]
+};
+
+// A state row's columns lie over LQ lanes of VEC each; a wavefront holds 64 / LQ rows at a time, WV wavefronts share a state, NR rows a
+// lane.  Four wavefronts a workgroup; blockIdx.y walks the columns where a row is wider than LQ VEC.
+template <class IO, int VEC, int LQ, int NR, int WV>
+__global__ __launch_bounds__(256) void delta_step_kernel(StepArgs a) {
+  constexpr int TEAMS = 4 / WV, RG = 64 / LQ * WV;         // states a workgroup, rows at a time
+  __shared__ float qk[TEAMS][2][128 + 4];
+  __shared__ float red[TEAMS][WV][3][LQ * VEC];
+  const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, team = wave / WV, w = wave % WV;
+  const int64_t p = a.p0 + (int64_t)blockIdx.x * TEAMS + team;
+  const bool live = p < a.P;
+  const int64_t pc = live ? p : 0, bn = pc / a.H;
+  const int h = (int)(pc - bn * a.H), kh = h / a.rep;
+  const int64_t b = bn / a.N, n = bn - b * a.N;
+  const int col = (int)blockIdx.y * LQ * VEC + (lane % LQ) * VEC;      // first column of this lane
+  const int row0 = w * (64 / LQ) + lane / LQ;
+  float* S = a.state + pc * a.K * a.V;
+  const bool mine = live && col < a.V;                    // (VEC divides V)
+
+  float s[NR][VEC];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int row = row0 + i * RG;
+    if (mine && row < a.K) pgt_ldv<VEC>(S + (int64_t)row * a.V + col, s[i]);
+    else
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) s[i][c] = 0.f;
+  }
+  const IO* kp = reinterpret_cast<const IO*>(a.k.p) + b * a.k.sb + n * a.k.sn + kh * a.k.sh;
+  const IO* qp = reinterpret_cast<const IO*>(a.q.p) + b * a.q.sb + n * a.q.sn + kh * a.q.sh;
+  const IO* vp = reinterpret_cast<const IO*>(a.v.p) + b * a.v.sb + n * a.v.sn + h * a.v.sh;
+  const float g = reinterpret_cast<const float*>(a.g.p)[b * a.g.sb + n * a.g.sn + h * a.g.sh];
+  const float beta = reinterpret_cast<const float*>(a.beta.p)[b * a.beta.sb + n * a.beta.sn + h * a.beta.sh];
+  for (int i = w * 64 + lane; i < 128; i += 64 * WV) {
+    qk[team][0][i] = i < a.K ? to_f32(kp[i]) : 0.f;
+    qk[team][1][i] = i < a.K ? to_f32(qp[i]) * a.scale : 0.f;
+  }
+  float v[VEC];
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) v[c] = col + c < a.V ? to_f32(vp[col + c]) : 0.f;
+  const float alpha = expf(g);
+  __syncthreads();
+  float ks[VEC], qs[VEC], dot = 0.f;
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) ks[c] = qs[c] = 0.f;
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int row = row0 + i * RG;
+    const float kr = row < 128 ? qk[team][0][row] : 0.f, qr = row < 128 ? qk[team][1][row] : 0.f;
+    dot = fmaf(kr, qr, dot);
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+      s[i][c] *= alpha;
+      ks[c] = fmaf(kr, s[i][c], ks[c]);
+      qs[c] = fmaf(qr, s[i][c], qs[c]);
+    }
+  }
+#pragma unroll
+  for (int m = LQ; m < 64; m <<= 1) {
+    dot += __shfl_xor(dot, m);
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) { ks[c] += __shfl_xor(ks[c], m); qs[c] += __shfl_xor(qs[c], m); }
+  }
+  if constexpr (WV > 1) {
+    if (lane < LQ) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        red[team][w][0][lane * VEC + c] = ks[c];
+        red[team][w][1][lane * VEC + c] = qs[c];
+        red[team][w][2][lane * VEC + c] = dot;
+      }
+    }
+    __syncthreads();
+    dot = 0.f;
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+      ks[c] = qs[c] = 0.f;
+#pragma unroll
+      for (int u = 0; u < WV; ++u) {
+        ks[c] += red[team][u][0][(lane % LQ) * VEC + c];
+        qs[c] += red[team][u][1][(lane % LQ) * VEC + c];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < WV; ++u) dot += red[team][u][2][0];
+  }
+  if (!mine) return;
+  float u[VEC];
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) u[c] = beta * (v[c] - ks[c]);
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int row = row0 + i * RG;
+    if (row < a.K) {
+      const float kr = qk[team][0][row];
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) s[i][c] = fmaf(kr, u[c], s[i][c]);
+      pgt_stv<VEC>(S + (int64_t)row * a.V + col, s[i]);
+    }
+  }
+  if (w == 0 && lane < LQ) {
+    IO* o = reinterpret_cast<IO*>(a.o) + p * a.V + col;
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) o[c] = from_f32<IO>(fmaf(dot, u[c], qs[c]));
+  }
+}
+
+template <class IO, int VEC, int LQ, int NR, int WV> void go(const StepArgs& a0, pgt_stream_t stream) {
+  StepArgs a = a0;
+  const int64_t most = (int64_t)1 << 22;
+  for (int64_t p0 = 0; p0 < a.P; p0 += most * (4 / WV)) {
+    a.p0 = p0;
+    const int64_t wgs = pgt_cdiv(a.P - p0, 4 / WV);
+    const dim3 grid((unsigned)(wgs < most ? wgs : most), (unsigned)((a.V + LQ * VEC - 1) / (LQ * VEC)));
+    PGT_LAUNCH((delta_step_kernel<IO, VEC, LQ, NR, WV>), grid, dim3(256), stream, a);
+  }
+}
+template <class IO> void pick(const StepArgs& a, bool vec, pgt_stream_t stream) {
+  const int kd = a.K <= 16 ? 16 : a.K <= 32 ? 32 : a.K <= 64 ? 64 : 128;
+#define PGT_STEP(VEC_, LQ_, N16, W16, N32, W32, N64, W64, N128, W128)      \
+  do {                                                                     \
+    if (kd == 16) go<IO, VEC_, LQ_, N16, W16>(a, stream);                  \
+    else if (kd == 32) go<IO, VEC_, LQ_, N32, W32>(a, stream);             \
+    else if (kd == 64) go<IO, VEC_, LQ_, N64, W64>(a, stream);             \
+    else go<IO, VEC_, LQ_, N128, W128>(a, stream);                         \
+  } while (0)
+  // (rows a lane, wavefronts a state) by key width: LQ NR WV = kd 64 / .. , at most sixteen rows of 16 bytes in flight a lane
+  if (!vec) PGT_STEP(1, 16, 4, 1, 8, 1, 16, 1, 16, 2);
+  else if (a.V <= 16) PGT_STEP(4, 4, 1, 1, 2, 1, 4, 1, 8, 1);
+  else if (a.V <= 32) PGT_STEP(4, 8, 2, 1, 4, 1, 8, 1, 16, 1);
+  else if (a.V <= 64) PGT_STEP(4, 16, 4, 1, 8, 1, 16, 1, 16, 2);
+  else PGT_STEP(4, 32, 8, 1, 16, 1, 16, 2, 16, 4);
+#undef PGT_STEP
+}
+
+}  // namespace
+
+extern "C" int pgt_gated_delta_step(const pgt_delta_dims* d, const pgt_seq_view* q, const pgt_seq_view* k, const pgt_seq_view* v,
+                                    const pgt_seq_view* g, const pgt_seq_view* beta, float* state, void* o, pgt_stream_t stream) {
+  Shape s;
+  if (int rc = pgt_delta_shape(d, "pgt_gated_delta_step", &s)) return rc;
+  PGT_REQUIRE(d->steps == 1 && d->lengths == nullptr, "pgt_gated_delta_step: one step, no lengths");
+  if (s.P == 0) return PGT_OK;
+  PGT_REQUIRE(q && k && v && g && beta && q->data && k->data && v->data && g->data && beta->data && state && o, "pgt_gated_delta_step: null pointer");
+  StepArgs a;
+  a.P = s.P; a.p0 = 0; a.N = s.N; a.H = s.H; a.rep = s.rep; a.K = s.K; a.V = s.V; a.scale = s.scale;
+  a.q = pgt_delta_view(q); a.k = pgt_delta_view(k); a.v = pgt_delta_view(v); a.g = pgt_delta_view(g); a.beta = pgt_delta_view(beta);
+  a.state = state; a.o = o;
+  const bool vec = s.V % 4 == 0 && pgt_aligned(state, 16);
+  if (d->dtype == PGT_DT_F32) pick<float>(a, vec, stream);
+  else if (d->dtype == PGT_DT_BF16) pick<bf16>(a, vec, stream);
+  else pick<f16>(a, vec, stream);
+  return pgt_check_launch("pgt_gated_delta_step");
+}

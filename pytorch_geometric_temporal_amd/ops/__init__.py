@@ -12,6 +12,7 @@ One module per model family (round 5 kept all of this in one 2 800-line file):
     astgcn    ASTGCN / MSTGCN: attention scores, batched products, ChebConvAttention
     evolve    EvolveGCN-H / -O weight evolution, the small-graph GCN layer
     stconv    STConv: TemporalConv, node-wise batch norm
+    delta     gated delta rule: sequences and single steps
     generic   aggregation / linear / read-out Functions shared by the families
 
 `ops.NAME` is the public spelling of every name below, as before.  The package is also where the SWITCHES are flipped
@@ -22,9 +23,9 @@ imported it — so the code that reads the switch sees it whichever module it li
 import sys
 import types
 
-from . import _graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv
+from . import _graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv, delta
 
-_FAMILIES = (_graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv)
+_FAMILIES = (_graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv, delta)
 
 for _m in _FAMILIES:
     for _k, _v in vars(_m).items():

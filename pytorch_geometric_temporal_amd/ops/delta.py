@@ -1,0 +1,174 @@
+"""Gated delta rule: whole sequences with gradients, and one step with the state in place.
+(One family of `pytorch_geometric_temporal_amd.ops`; the package re-exports every name and forwards writes to its switches.)
+"""
+import ctypes
+
+import torch
+
+from .. import _lib
+from .._lib import DeltaDimsStruct, SeqViewStruct, check_tensor, ptr, stream_of
+
+F32 = torch.float32
+
+from ._core import KERNEL_TIMER, _timed
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MAX_HEAD_WIDTH = 128
+
+
+def _view(t, step):
+    """pgt_seq_view of [B, T, N, H(, C)] (step) or [B, N, H(, C)]."""
+    st = t.stride()
+    v = SeqViewStruct(t.data_ptr(), st[0], st[1], st[2], st[3]) if step else SeqViewStruct(t.data_ptr(), st[0], 0, st[1], st[2])
+    return ctypes.byref(v)
+
+
+def _last_axis_contiguous(t):
+    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _check(lib, what, q, k, v, g, beta, lead):
+    """Types, devices and shapes of an operator's inputs; returns (k_heads, heads, key, value)."""
+    if not isinstance(v, torch.Tensor) or v.dtype not in DTYPES:
+        raise TypeError(f"{what}: v must be a float32, bfloat16 or float16 tensor, got {getattr(v, 'dtype', type(v))}")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        check_tensor(lib, t, f"{what}: {name}", v.dtype)
+    for t, name in ((g, "g"), (beta, "beta")):
+        check_tensor(lib, t, f"{what}: {name}")
+    if v.dim() != lead + 2 or q.dim() != lead + 2 or q.shape[:lead] != v.shape[:lead]:
+        axes = "[batch, steps, nodes, heads, width]" if lead == 3 else "[batch, nodes, heads, width]"
+        raise ValueError(f"{what}: q, k, v must be {axes} with the same leading axes, got q {tuple(q.shape)}, v {tuple(v.shape)}")
+    if k.shape != q.shape:
+        raise ValueError(f"{what}: k {tuple(k.shape)} must have q's shape {tuple(q.shape)}")
+    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
+        raise ValueError(f"{what}: g {tuple(g.shape)} and beta {tuple(beta.shape)} must be {tuple(v.shape[:-1])}")
+    Hk, K, H, V = q.size(-2), q.size(-1), v.size(-2), v.size(-1)
+    if Hk < 1 or H < 1 or H % Hk:
+        raise ValueError(f"{what}: {H} value heads do not divide over {Hk} key heads")
+    if not (1 <= K <= MAX_HEAD_WIDTH and 1 <= V <= MAX_HEAD_WIDTH):
+        raise ValueError(f"{what}: head widths must be 1 .. {MAX_HEAD_WIDTH}, got key {K}, value {V}")
+    for t in (q, k, g, beta):
+        if t.device != v.device:
+            raise ValueError(f"{what}: inputs on {t.device} and {v.device}")
+    return Hk, H, K, V
+
+
+def _check_state(lib, what, name, t, shape, device):
+    check_tensor(lib, t, f"{what}: {name}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{what}: {name} must be {shape}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, the inputs on {device}")
+
+
+class GatedDeltaFunction(torch.autograd.Function):
+    """pgt_gated_delta_fwd / pgt_gated_delta_bwd.  For the adjoint the forward pass keeps the misses e and the state before every
+    sixteenth step; with few sequences and many steps also the segments' transitions (pgt_gated_delta_segments)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, start, lengths, scale):
+        lib = _lib.get_lib()
+        B, T, N, H, V = v.shape
+        Hk, K = q.shape[3:]
+        dev, P = v.device, B * N * H
+        dims = DeltaDimsStruct(B, T, N, Hk, H, K, V, DTYPES[v.dtype], scale, ptr(lengths))
+        segs = lib._pgt_gated_delta_segments(ctypes.byref(dims))
+        if segs < 0:
+            raise _lib.PgtError(f"gated_delta_rule: {lib.last_error()}")
+        need = any(ctx.needs_input_grad)
+        o = torch.empty(B, T, N, H, V, dtype=v.dtype, device=dev)
+        last = torch.empty(B, N, H, K, V, dtype=F32, device=dev)
+        e = torch.empty(B, T, N, H, V, dtype=F32, device=dev) if need else None
+        states = torch.empty(P, max((T + 15) // 16 - 1, 0), K, V, dtype=F32, device=dev) if need else None
+        seg_start = torch.empty(P, segs - 1, K, V, dtype=F32, device=dev) if segs > 1 else None
+        seg_trans = torch.empty(P, segs - 2, K, K, dtype=F32, device=dev) if segs > 1 else None
+        _timed("gated_delta", 7.0 * P * T * K * V if KERNEL_TIMER else 0, lambda: lib.call(
+            "pgt_gated_delta_fwd", ctypes.byref(dims), _view(q, True), _view(k, True), _view(v, True), _view(g, True), _view(beta, True),
+            ptr(start), ptr(o), ptr(last), ptr(e), ptr(states), ptr(seg_start), ptr(seg_trans), stream_of(lib, v)))
+        if need:
+            ctx.save_for_backward(q, k, g, beta, start, lengths, e, states, seg_trans)
+            ctx.dims = (B, T, N, Hk, H, K, V, v.dtype, scale, segs)
+        ctx.set_materialize_grads(False)
+        return o, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, d_last):
+        lib = _lib.get_lib()
+        q, k, g, beta, start, lengths, e, states, seg_trans = ctx.saved_tensors
+        B, T, N, Hk, H, K, V, dtype, scale, segs = ctx.dims
+        dev, P = q.device, B * N * H
+        if d_o is None and d_last is None:
+            return (None,) * 8
+        d_o = torch.zeros(B, T, N, H, V, dtype=dtype, device=dev) if d_o is None else d_o.contiguous()
+        d_last = None if d_last is None else d_last.contiguous()
+        dq = torch.empty(B, T, N, Hk, K, dtype=dtype, device=dev)
+        dk = torch.empty_like(dq)
+        dv = torch.empty(B, T, N, H, V, dtype=dtype, device=dev)
+        dg = torch.empty(B, T, N, H, dtype=F32, device=dev)
+        dbeta = torch.empty_like(dg)
+        d_start = torch.empty(B, N, H, K, V, dtype=F32, device=dev) if start is not None and ctx.needs_input_grad[5] else None
+        head_ws = torch.empty(2, P * T * K, dtype=F32, device=dev) if H > Hk else None
+        seg_end = torch.empty(P, segs - 1, K, V, dtype=F32, device=dev) if segs > 1 else None
+        dims = DeltaDimsStruct(B, T, N, Hk, H, K, V, DTYPES[dtype], scale, ptr(lengths))
+        _timed("gated_delta_bwd", 14.0 * P * T * K * V if KERNEL_TIMER else 0, lambda: lib.call(
+            "pgt_gated_delta_bwd", ctypes.byref(dims), _view(q, True), _view(k, True), _view(g, True), _view(beta, True), ptr(start),
+            ptr(e), ptr(states), ptr(seg_trans), ptr(d_o), ptr(d_last), ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(dbeta), ptr(d_start),
+            ptr(head_ws), ptr(seg_end), stream_of(lib, q)))
+        return dq, dk, dv, dg, dbeta, d_start, None, None
+
+
+def gated_delta_rule(q, k, v, g, beta, initial_state=None, lengths=None, scale=None):
+    """The gated delta rule along the steps of every (sample, node, head), with state S [key, value]:
+
+        S_t = exp(g_t) S_{t-1} + k_t u_t^T,   u_t = beta_t (v_t - exp(g_t) S_{t-1}^T k_t),   o_t = scale S_t^T q_t
+
+    q, k [B, T, N, Hk, K], v [B, T, N, H, V]: float32, bfloat16 or float16, one type; g (log decay, <= 0), beta [B, T, N, H]: float32.
+    H is a multiple of Hk: value head h reads key head h // (H // Hk).  K, V: 1 .. 128.  Any strides (slices of one projection are
+    read in place as long as the last axis is contiguous).  q and k are used as they are: normalise them before.
+    initial_state [B, N, H, K, V] float32 or None (zeros).  lengths: int32 / int64 [B] or [B, N] on the same device, how many steps of each
+    sequence there are: the steps behind are not looked at, their outputs and gradients are 0 (values outside 0 .. T are clamped).
+    scale: default K ** -0.5.  g = -inf forgets the state.
+
+    Returns (o [B, T, N, H, V] in v's type, final_state [B, N, H, K, V] float32), both differentiable (once).  Products and states are
+    held in float32 whatever the inputs' type; results and gradients are bitwise reproducible."""
+    lib = _lib.get_lib()
+    what = "gated_delta_rule"
+    Hk, H, K, V = _check(lib, what, q, k, v, g, beta, 3)
+    B, T, N = v.shape[:3]
+    if initial_state is not None:
+        _check_state(lib, what, "initial_state", initial_state, (B, N, H, K, V), v.device)
+        initial_state = initial_state.contiguous()
+    if lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"{what}: lengths must be an int32 or int64 tensor")
+        if lengths.device != v.device:
+            raise ValueError(f"{what}: lengths are on {lengths.device}, the inputs on {v.device}")
+        if tuple(lengths.shape) not in ((B,), (B, N)):
+            raise ValueError(f"{what}: lengths must be [{B}] or [{B}, {N}], got {tuple(lengths.shape)}")
+        lengths = (lengths if lengths.dim() == 2 else lengths[:, None]).clamp(0, T).to(torch.int32).expand(B, N).contiguous()
+    scale = float(K) ** -0.5 if scale is None else float(scale)
+    with torch.cuda.device_of(v):
+        return GatedDeltaFunction.apply(*(_last_axis_contiguous(t) for t in (q, k, v)), g, beta, initial_state, lengths, scale)
+
+
+def gated_delta_step(q, k, v, g, beta, state, scale=None):
+    """One step of `gated_delta_rule` for serving: q, k [B, N, Hk, K], v [B, N, H, V], g, beta [B, N, H], state [B, N, H, K, V] float32
+    contiguous, UPDATED IN PLACE.  Returns o [B, N, H, V] in v's type.  Not differentiable (refused where a gradient is asked for)."""
+    lib = _lib.get_lib()
+    what = "gated_delta_step"
+    Hk, H, K, V = _check(lib, what, q, k, v, g, beta, 2)
+    B, N = v.shape[:2]
+    _check_state(lib, what, "state", state, (B, N, H, K, V), v.device)
+    if not state.is_contiguous():
+        raise ValueError(f"{what}: state must be contiguous (it is updated in place)")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or use gated_delta_rule")
+    q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
+    o = torch.empty(B, N, H, V, dtype=v.dtype, device=v.device)
+    dims = DeltaDimsStruct(B, 1, N, Hk, H, K, V, DTYPES[v.dtype], float(K) ** -0.5 if scale is None else float(scale), None)
+    with torch.cuda.device_of(v):
+        _timed("gated_delta_step", 8.0 * state.numel() if KERNEL_TIMER else 0, lambda: lib.call(
+            "pgt_gated_delta_step", ctypes.byref(dims), _view(q, False), _view(k, False), _view(v, False), _view(g, False),
+            _view(beta, False), ptr(state), ptr(o), stream_of(lib, v)))
+    return o

@@ -1,0 +1,58 @@
+// TEST INFRASTRUCTURE (CPU test double only, never part of libpgt_hip.so): the platform layer of csrc/delta_common.h in plain C++.
+// On the device these operations are gfx950 instructions (v_mfma_f32_16x16x4_f32, DPP moves inside a row of sixteen lanes, the
+// LDS-only barrier, fp16 / bf16 conversions); here they run on the wavefront's 64 fibers.
+#pragma once
+struct gd_f4 {
+  float v[4];
+  float& operator[](int i) { return v[i]; }
+  const float& operator[](int i) const { return v[i]; }
+};
+// v_mfma_f32_16x16x4_f32: lane l holds A[i = l % 16][k = l / 16] and B[k = l / 16][j = l % 16]; D: col = l % 16, row = 4 (l / 16) + reg
+static inline gd_f4 gd_mfma(float a, float b, gd_f4 c) {
+  pgt_emu::State& st = pgt_emu::S();
+  const unsigned w = st.cur / 64, lane = st.cur % 64;
+  st.w_slot[w * 64 + lane] = pgt_emu::to_bits(a);
+  st.w_slot2[w * 64 + lane] = pgt_emu::to_bits(b);
+  pgt_emu::wave_barrier();
+  const unsigned col = lane & 15;
+  for (int r = 0; r < 4; ++r) {
+    const unsigned row = 4 * (lane >> 4) + r;
+    float acc = c[r];
+    for (int k = 0; k < 4; ++k)
+      acc = fmaf(pgt_emu::from_bits<float>(st.w_slot[w * 64 + row + 16 * k]), pgt_emu::from_bits<float>(st.w_slot2[w * 64 + col + 16 * k]), acc);
+    c[r] = acc;
+  }
+  pgt_emu::wave_barrier();
+  return c;
+}
+template <int J> static inline float gd_bcast16(float x) { return __shfl(x, (__lane_id() & 48) | J); }
+template <int N> static inline float gd_ror16(float x) { return __shfl(x, (__lane_id() & 48) | ((__lane_id() - N) & 15)); }
+template <int N> static inline double gd_shr16(double x) {          // lane i takes lane i - N of its row, 0 where there is none
+  const double y = __shfl(x, (__lane_id() & 48) | ((__lane_id() - N) & 15));
+  return (__lane_id() & 15) >= N ? y : 0.0;
+}
+static inline void gd_wave_sync() { pgt_emu::wave_barrier(); }
+static inline void gd_block_sync() { __syncthreads(); }
+static inline float gd_as_float(uint32_t u) { float f; memcpy(&f, &u, 4); return f; }
+static inline uint32_t gd_as_uint(float f) { uint32_t u; memcpy(&u, &f, 4); return u; }
+static inline uint16_t gd_to_bf16(float x) {
+  uint32_t u = gd_as_uint(x);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
+  return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+static inline float gd_from_f16(uint16_t h) {
+  const uint32_t s = (uint32_t)(h & 0x8000u) << 16, e = (h >> 10) & 31u, m = h & 1023u;
+  if (e == 31) return gd_as_float(s | 0x7f800000u | (m << 13));
+  if (e == 0) { const float f = ldexpf((float)m, -24); return s ? -f : f; }
+  return gd_as_float(s | ((e + 112u) << 23) | (m << 13));
+}
+static inline uint16_t gd_to_f16(float x) {
+  const uint32_t u = gd_as_uint(x), s = (u >> 16) & 0x8000u;
+  const float a = fabsf(x);
+  if (!(a == a)) return (uint16_t)(s | 0x7e00u);
+  if (a >= 65520.f) return (uint16_t)(s | 0x7c00u);
+  if (a < 6.103515625e-05f) return (uint16_t)(s | (uint32_t)nearbyintf(ldexpf(a, 24)));      // subnormal (or rounds up to the least normal)
+  const uint32_t v = gd_as_uint(a);
+  const uint32_t r = v + 0xfffu + ((v >> 13) & 1u);
+  return (uint16_t)(s | ((r >> 13) - (112u << 10)));
+}
