@@ -754,6 +754,23 @@ int pgt_gated_delta_bwd(const pgt_delta_dims* dims, const pgt_seq_view* q, const
 int pgt_gated_delta_step(const pgt_delta_dims* dims, const pgt_seq_view* q, const pgt_seq_view* k, const pgt_seq_view* v,
                          const pgt_seq_view* g, const pgt_seq_view* beta, float* state, void* o, pgt_stream_t stream);
 
+/* Group norm with an activation on channels-last tensors (csrc/group_norm.hip): x [batch, rows, channels] contiguous, `rows` everything
+ * between the sample axis and the channels, statistics per (sample, group of channels / groups neighbouring channels) over rows and channels:
+ *   y = act(weight (x - mean) rstd + bias),  rstd = 1 / sqrt(var + eps), var over all of the group's values (biased).
+ * x, y, dy, dx in one type (PGT_DT_*); weight, bias [channels] fp32 (NULL: 1, 0); act PGT_ACT_*.  stats [batch, groups, 2] (mean, rstd):
+ * written by the forward pass, read by the adjoint (rows == 1 and channels / groups <= 512: may be NULL in both).  ws: pgt_group_norm_ws_floats
+ * floats (adjoint != 0: for the adjoint).  dx, dweight, dbias: NULL where not wanted; the parameter gradients are sums in a fixed order. */
+#define PGT_ACT_NONE 0
+#define PGT_ACT_RELU 1
+#define PGT_ACT_SILU 2
+int64_t pgt_group_norm_ws_floats(int64_t batch, int64_t rows, int64_t channels, int64_t groups, int dtype, int adjoint);
+int pgt_group_norm_act(const void* x, int64_t batch, int64_t rows, int64_t channels, int64_t groups, int dtype, const float* weight,
+                       const float* bias, float eps, int act, void* y, float* stats, float* ws, int64_t ws_floats,
+                       pgt_stream_t stream);
+int pgt_group_norm_act_bwd(const void* x, const void* dy, const float* stats, int64_t batch, int64_t rows, int64_t channels,
+                           int64_t groups, int dtype, const float* weight, const float* bias, float eps, int act, void* dx,
+                           float* dweight, float* dbias, float* ws, int64_t ws_floats, pgt_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,7 +14,7 @@ INCLUDE = os.path.join(ROOT, "include")
 
 SOURCES = ["pgt_core.hip", "spmm.hip", "dconv_slab.hip", "gemm.hip", "gemm_bx.hip", "elementwise.hip",
            "graph_prep.hip", "attention.hip", "evolve.hip", "small_cell.hip", "small_gcn.hip", "tconv.hip", "tgcn.hip", "seq_small.hip", "tgcn_cell.hip", "tile_order.hip", "readout.hip", "seq64.hip",
-           "delta_fwd.hip", "delta_bwd.hip", "delta_step.hip"]
+           "delta_fwd.hip", "delta_bwd.hip", "delta_step.hip", "group_norm.hip"]
 HEADERS = ["pgt_common.h", "delta_common.h"]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32.  The compiler makes them from ordinary float code, and some of their forms have
 # given wrong results on MI355X now and then.  (The host pass warns that it does not know the feature.)

@@ -211,6 +211,11 @@ PROTOTYPES = {
     "pgt_gated_delta_bwd": (c_int, [c_dims, c_view, c_view, c_view, c_view, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr,
                                     c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr, c_ptr]),
     "pgt_gated_delta_step": (c_int, [c_dims, c_view, c_view, c_view, c_view, c_view, c_ptr, c_ptr, c_ptr]),
+    "pgt_group_norm_ws_floats": (c_i64, [c_i64, c_i64, c_i64, c_i64, c_int, c_int]),
+    "pgt_group_norm_act": (c_int, [c_ptr, c_i64, c_i64, c_i64, c_i64, c_int, c_ptr, c_ptr, c_f32, c_int, c_ptr, c_ptr, c_ptr, c_i64,
+                                   c_ptr]),
+    "pgt_group_norm_act_bwd": (c_int, [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i64, c_int, c_ptr, c_ptr, c_f32, c_int, c_ptr,
+                                       c_ptr, c_ptr, c_ptr, c_i64, c_ptr]),
 }
 
 EXPECTED_ABI = 18

@@ -35,6 +35,19 @@ template <int N> __device__ __forceinline__ double gd_shr16(double x) {      // 
   const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), 0x110 + N, 0xf, 0xf, true);
   return __longlong_as_double(((uint64_t)hi << 32) | lo);
 }
+// the sum over an aligned cluster of 1, 2, 4, .. 64 lanes (the same count in every lane), in every lane of it: DPP quad_perm, half and whole
+// row mirrors (the partners hold equal partial sums by then), ds_bpermute beyond a row
+__device__ __forceinline__ float gd_xsum(float x, int lanes) {
+  if (lanes > 1) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true));
+  if (lanes > 2) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4e, 0xf, 0xf, true));
+  if (lanes > 4) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xf, 0xf, true));
+  if (lanes > 8) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xf, 0xf, true));
+  if (lanes > 16) x += __shfl_xor(x, 16);
+  if (lanes > 32) x += __shfl_xor(x, 32);
+  return x;
+}
+__device__ __forceinline__ float gd_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ __forceinline__ float gd_exp(float x) { return __expf(x); }
 // LDS hand-off inside one wavefront / inside the workgroup (global loads and stores stay in flight across it)
 __device__ __forceinline__ void gd_wave_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void gd_block_sync() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }

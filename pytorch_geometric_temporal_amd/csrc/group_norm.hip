@@ -1,0 +1,609 @@
+// Group norm with an activation on channels-last tensors x [B, S, C]: statistics per (sample, group of Cg = C / G channels) over the S rows.
+//   z = w (x - mean) rstd + b,  y = act(z);      xh = (x - mean) rstd,  dz = dy act'(z)
+//   dw_c = sum dz xh,  db_c = sum dz,  dx = rstd (w dz - (s1 + xh s2) / n),  s1 = sum w dz, s2 = sum w dz xh over the group's n = S Cg values.
+// Everything is bound by memory: x (and dy) in, y (dx) out.
+//   S = 1 (a row by itself, a group to a head): each (row, group) is Cg neighbouring values; a cluster of lanes holds them in registers,
+//     so one pass over the data gives statistics and result, in the adjoint too (the statistics are taken again, not stored).
+//   S > 1: a sample does not fit a CU.  Two launches: sums per channel and slice of rows, then the result, every workgroup joining
+//     the slices' sums itself (they are few and in cache).  Threads keep their channels, so weights and statistics sit in registers.
+// Sums are fp32; the variance is taken from deviations from a value of the same channel (S > 1: the sample's first row) or
+// from the mean itself (S = 1), never as a difference of large squares.  No atomics: the order of every sum is fixed.
+#include "delta_common.h"
+
+using namespace gd;
+
+namespace {
+
+template <class IO, int VEC> struct alignas(sizeof(IO) * VEC) Pack { IO v[VEC]; };
+template <class IO, int VEC> __device__ __forceinline__ void get(const IO* p, float (&x)[VEC]) {
+  const Pack<IO, VEC> t = *reinterpret_cast<const Pack<IO, VEC>*>(p);
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) x[c] = to_f32(t.v[c]);
+}
+template <class IO, int VEC> __device__ __forceinline__ void put(IO* p, const float (&x)[VEC]) {
+  Pack<IO, VEC> t;
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) t.v[c] = from_f32<IO>(x[c]);
+  *reinterpret_cast<Pack<IO, VEC>*>(p) = t;
+}
+// exp and rcp of the hardware: silu and its slope to about 3e-7 of their scale
+template <int VEC> __device__ __forceinline__ void activate(float (&z)[VEC], int act) {
+  if (act == PGT_ACT_RELU) {
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) z[c] = z[c] < 0.f ? 0.f : z[c];
+  } else if (act == PGT_ACT_SILU) {
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) z[c] *= gd_rcp(1.f + gd_exp(-z[c]));
+  }
+}
+// g <- g act'(z)
+template <int VEC> __device__ __forceinline__ void slope(float (&g)[VEC], const float (&z)[VEC], int act) {
+  if (act == PGT_ACT_RELU) {
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) g[c] = z[c] > 0.f ? g[c] : 0.f;
+  } else if (act == PGT_ACT_SILU) {
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+      const float s = gd_rcp(1.f + gd_exp(-z[c]));
+      g[c] *= s * (1.f + z[c] * (1.f - s));
+    }
+  }
+}
+
+struct NormArgs {
+  const void* x; const void* dy; void* y;                  // y: dx in the adjoint
+  const float* w; const float* b;
+  float* stats; float* ws;
+  float* dw; float* db;
+  int64_t B, S, b0;              // b0: first sample of this launch
+  int C, G, Cg, act, slices, lanes, groups_y, reps;
+  int64_t slice_rows;
+  float eps;
+};
+
+// ---- S = 1.  A cluster of a.lanes lanes owns group g of rows row, row + step, ..; blockIdx.y walks the groups where a workgroup does not
+// cover them all.
+template <class IO, int VEC, int NV, bool BWD>
+__global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
+  __shared__ __attribute__((aligned(16))) float acc[2][256 * VEC];
+  const int tid = (int)threadIdx.x, lanes = a.lanes, cl = tid / lanes, lane = tid % lanes;
+  const int g = (int)blockIdx.y * a.groups_y + cl % a.groups_y, rep = cl / a.groups_y;
+  const bool mine = rep < a.reps && g < a.G;
+  float w[NV][VEC], b[NV][VEC];
+  bool on[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int e = (lane + lanes * j) * VEC;
+    on[j] = mine && e < a.Cg;
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+      w[j][c] = on[j] && a.w ? a.w[g * a.Cg + e + c] : 1.f;
+      b[j][c] = on[j] && a.b ? a.b[g * a.Cg + e + c] : 0.f;
+    }
+  }
+  float dw[BWD ? NV : 1][VEC], db[BWD ? NV : 1][VEC];
+  if (BWD) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) dw[j][c] = db[j][c] = 0.f;
+  }
+  const float inv_n = 1.f / (float)a.Cg;
+  const int64_t step = (int64_t)gridDim.x * a.reps;
+  for (int64_t row0 = (int64_t)blockIdx.x * a.reps; row0 < a.B; row0 += step) {
+    const int64_t row = row0 + rep, at = row * a.C + (int64_t)g * a.Cg;
+    const bool in = row < a.B;
+    float x[NV][VEC], d[BWD ? NV : 1][VEC];
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e = (lane + lanes * j) * VEC;
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) x[j][c] = 0.f;
+      if (on[j] && in) get<IO, VEC>(reinterpret_cast<const IO*>(a.x) + at + e, x[j]);
+      if (BWD) {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) d[j][c] = 0.f;
+        if (on[j] && in) get<IO, VEC>(reinterpret_cast<const IO*>(a.dy) + at + e, d[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) sum += x[j][c];
+    const float mean = gd_xsum(sum, lanes) * inv_n;
+    float sq = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        x[j][c] = on[j] ? x[j][c] - mean : 0.f;
+        sq = fmaf(x[j][c], x[j][c], sq);
+      }
+    const float rstd = 1.f / sqrtf(gd_xsum(sq, lanes) * inv_n + a.eps);
+    if (!BWD) {
+      if (a.stats && mine && in && lane == 0) {
+        a.stats[(row * a.G + g) * 2] = mean;
+        a.stats[(row * a.G + g) * 2 + 1] = rstd;
+      }
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) x[j][c] = fmaf(w[j][c], x[j][c] * rstd, b[j][c]);
+        activate<VEC>(x[j], a.act);
+        if (on[j] && in) put<IO, VEC>(reinterpret_cast<IO*>(a.y) + at + (lane + lanes * j) * VEC, x[j]);
+      }
+    } else {
+      float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float z[VEC];
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          x[j][c] *= rstd;
+          z[c] = fmaf(w[j][c], x[j][c], b[j][c]);
+        }
+        slope<VEC>(d[j], z, a.act);
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          db[j][c] += d[j][c];
+          dw[j][c] = fmaf(d[j][c], x[j][c], dw[j][c]);
+          d[j][c] *= w[j][c];
+          s1 += d[j][c];
+          s2 = fmaf(d[j][c], x[j][c], s2);
+        }
+      }
+      s1 = gd_xsum(s1, lanes) * inv_n;
+      s2 = gd_xsum(s2, lanes) * inv_n;
+      if (a.y) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) d[j][c] = rstd * (d[j][c] - s1 - x[j][c] * s2);
+          if (on[j] && in) put<IO, VEC>(reinterpret_cast<IO*>(a.y) + at + (lane + lanes * j) * VEC, d[j]);
+        }
+      }
+    }
+  }
+  if (BWD) {                                              // this workgroup's sums: over its clusters of the same group, in order
+    if (a.ws == nullptr) return;                          // (no parameter gradients wanted)
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) { acc[0][tid * VEC + c] = dw[j][c]; acc[1][tid * VEC + c] = db[j][c]; }
+      __syncthreads();
+      const int e = (lane + lanes * j) * VEC;
+      if (rep == 0 && on[j]) {
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+          for (int c = 0; c < VEC; ++c) {
+            float t = 0.f;
+            for (int r = 0; r < a.reps; ++r) t += acc[q][(tid + r * a.groups_y * lanes) * VEC + c];
+            a.ws[((int64_t)blockIdx.x * 2 + q) * a.C + g * a.Cg + e + c] = t;
+          }
+      }
+    }
+  }
+}
+
+// ---- S > 1.  Thread (tr, tq) walks rows tr, tr + RP, .. of its slice at vector tq of the row; blockIdx.z walks rows wider than 256 vectors.
+__device__ __forceinline__ int64_t sample_of(const NormArgs& a) { return a.b0 + blockIdx.y; }
+struct Place { int nq, tq, tr, rp; bool on; int c0; int64_t r0, r1; };
+template <int VEC> __device__ __forceinline__ Place place(const NormArgs& a) {
+  Place p;
+  const int total = a.C / VEC, tid = (int)threadIdx.x;
+  p.nq = total - (int)blockIdx.z * 256;
+  p.nq = p.nq > 256 ? 256 : p.nq;
+  p.rp = 256 / p.nq;
+  p.tr = tid / p.nq;
+  p.tq = tid - p.tr * p.nq;
+  p.on = p.tr < p.rp;
+  p.c0 = ((int)blockIdx.z * 256 + p.tq) * VEC;
+  p.r0 = (int64_t)blockIdx.x * a.slice_rows;
+  p.r1 = p.r0 + a.slice_rows < a.S ? p.r0 + a.slice_rows : a.S;
+  return p;
+}
+// this workgroup's sums over its rows: ws[b][slice][2][C]
+template <int VEC> __device__ __forceinline__ void slice_sums(const NormArgs& a, const Place& p, float (&s)[2][VEC], float* lds) {
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) lds[(int)threadIdx.x * VEC + c] = p.on ? s[q][c] : 0.f;
+    __syncthreads();
+    for (int e = (int)threadIdx.x; e < p.nq * VEC; e += 256) {
+      float t = 0.f;
+      for (int r = 0; r < p.rp; ++r) t += lds[r * p.nq * VEC + e];
+      a.ws[((sample_of(a) * a.slices + blockIdx.x) * 2 + q) * a.C + blockIdx.z * 256 * VEC + e] = t;
+    }
+  }
+}
+// the sums over a sample's slices of channel c
+__device__ __forceinline__ void channel_sums(const NormArgs& a, int c, float& s0, float& s1) {
+  s0 = s1 = 0.f;
+  const float* p = a.ws + sample_of(a) * a.slices * 2 * a.C + c;
+  for (int i = 0; i < a.slices; ++i) { s0 += p[(int64_t)(2 * i) * a.C]; s1 += p[(int64_t)(2 * i + 1) * a.C]; }
+}
+
+template <class IO, int VEC>
+__global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[256 * VEC];
+  const Place p = place<VEC>(a);
+  const IO* x = reinterpret_cast<const IO*>(a.x) + sample_of(a) * a.S * a.C + p.c0;
+  float s[2][VEC], piv[VEC];
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) s[0][c] = s[1][c] = 0.f;
+  if (p.on) {
+    get<IO, VEC>(x, piv);
+    int64_t r = p.r0 + p.tr;
+    for (; r + 3 * p.rp < p.r1; r += 4 * p.rp) {
+      float v[4][VEC];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) get<IO, VEC>(x + (r + u * p.rp) * a.C, v[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) {
+          const float d = v[u][c] - piv[c];
+          s[0][c] += d;
+          s[1][c] = fmaf(d, d, s[1][c]);
+        }
+    }
+    for (; r < p.r1; r += p.rp) {
+      float v[VEC];
+      get<IO, VEC>(x + r * a.C, v);
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) {
+        const float d = v[c] - piv[c];
+        s[0][c] += d;
+        s[1][c] = fmaf(d, d, s[1][c]);
+      }
+    }
+  }
+  slice_sums<VEC>(a, p, s, lds);
+}
+
+// Joins the sums of a sample: per group (mean, rstd) into st[g][2].  Channel c: mean m_c = pivot + s0 / S, squares about it s1 - s0^2 / S; the
+// group's squares are those plus S (m_c - mean)^2.  Two rounds over the group's channels, a wavefront to a group.
+template <class IO> __device__ __forceinline__ void join_stats(const NormArgs& a, float* st, int g0, int g1) {
+  const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+  const IO* x = reinterpret_cast<const IO*>(a.x) + sample_of(a) * a.S * a.C;
+  const float inv_s = 1.f / (float)a.S;
+  for (int g = g0 + wave; g < g1; g += 4) {
+    float sum = 0.f, sq = 0.f, m0 = 0.f;
+    const int c_lo = g * a.Cg;
+    for (int i = lane; i < a.Cg; i += 64) {
+      float s0, s1;
+      channel_sums(a, c_lo + i, s0, s1);
+      const float m = to_f32(x[c_lo + i]) + s0 * inv_s;
+      if (i == lane) m0 = m;
+      sum += m;
+      sq += s1 - s0 * (s0 * inv_s);
+    }
+    const float mean = gd_xsum(sum, 64) / (float)a.Cg;
+    float dev = 0.f;
+    for (int i = lane; i < a.Cg; i += 64) {
+      float m = m0;
+      if (i != lane) {
+        float s0, s1;
+        channel_sums(a, c_lo + i, s0, s1);
+        m = to_f32(x[c_lo + i]) + s0 * inv_s;
+      }
+      dev = fmaf(m - mean, m - mean, dev);
+    }
+    const float var = (gd_xsum(sq, 64) + (float)a.S * gd_xsum(dev, 64)) / ((float)a.S * (float)a.Cg);
+    if (lane == 0) {
+      st[2 * (g - g0)] = mean;
+      st[2 * (g - g0) + 1] = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
+    }
+  }
+}
+
+template <class IO, int VEC>
+__global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
+  __shared__ float st[2 * (256 * VEC + 2)];
+  const Place p = place<VEC>(a);
+  const int clo = (int)blockIdx.z * 256 * VEC, chi = clo + p.nq * VEC;
+  const int g0 = clo / a.Cg, g1 = (chi - 1) / a.Cg + 1;
+  join_stats<IO>(a, st, g0, g1);
+  __syncthreads();
+  if (a.stats && blockIdx.x == 0)
+    for (int i = (int)threadIdx.x; i < 2 * (g1 - g0); i += 256) a.stats[(sample_of(a) * a.G + g0) * 2 + i] = st[i];
+  if (!p.on) return;
+  float sc[VEC], mean[VEC], b[VEC];
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) {
+    const int g = (p.c0 + c) / a.Cg - g0;
+    mean[c] = st[2 * g];
+    sc[c] = st[2 * g + 1] * (a.w ? a.w[p.c0 + c] : 1.f);
+    b[c] = a.b ? a.b[p.c0 + c] : 0.f;
+  }
+  const int64_t base = sample_of(a) * a.S * a.C + p.c0;
+  const IO* x = reinterpret_cast<const IO*>(a.x) + base;
+  IO* y = reinterpret_cast<IO*>(a.y) + base;
+  int64_t r = p.r0 + p.tr;
+  for (; r + 3 * p.rp < p.r1; r += 4 * p.rp) {
+    float v[4][VEC];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) get<IO, VEC>(x + (r + u * p.rp) * a.C, v[u]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) v[u][c] = fmaf(sc[c], v[u][c] - mean[c], b[c]);
+      activate<VEC>(v[u], a.act);
+      put<IO, VEC>(y + (r + u * p.rp) * a.C, v[u]);
+    }
+  }
+  for (; r < p.r1; r += p.rp) {
+    float v[VEC];
+    get<IO, VEC>(x + r * a.C, v);
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) v[c] = fmaf(sc[c], v[c] - mean[c], b[c]);
+    activate<VEC>(v, a.act);
+    put<IO, VEC>(y + r * a.C, v);
+  }
+}
+
+// the adjoint's two launches: DX false: sums of dz xh (= dw) and dz (= db) by channel and slice; DX true: dx
+template <class IO, int VEC, bool DX>
+__global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
+  __shared__ __attribute__((aligned(16))) float lds[DX ? 2 * (256 * VEC + 2) : 256 * VEC];
+  const Place p = place<VEC>(a);
+  const int clo = (int)blockIdx.z * 256 * VEC, chi = clo + p.nq * VEC;
+  const int g0 = clo / a.Cg, g1 = (chi - 1) / a.Cg + 1;
+  if (DX) {
+    const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
+    const float inv_n = 1.f / ((float)a.S * (float)a.Cg);
+    for (int g = g0 + wave; g < g1; g += 4) {
+      float t1 = 0.f, t2 = 0.f;
+      for (int i = lane; i < a.Cg; i += 64) {
+        float dw, db;
+        channel_sums(a, g * a.Cg + i, dw, db);
+        const float w = a.w ? a.w[g * a.Cg + i] : 1.f;
+        t1 = fmaf(w, db, t1);
+        t2 = fmaf(w, dw, t2);
+      }
+      t1 = gd_xsum(t1, 64) * inv_n;
+      t2 = gd_xsum(t2, 64) * inv_n;
+      if (lane == 0) { lds[2 * (g - g0)] = t1; lds[2 * (g - g0) + 1] = t2; }
+    }
+    __syncthreads();
+    if (!p.on) return;
+  }
+  float w[VEC], b[VEC], mean[VEC], rstd[VEC], s1[VEC], s2[VEC], s[2][VEC];
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) {
+    w[c] = p.on && a.w ? a.w[p.c0 + c] : 1.f;
+    b[c] = p.on && a.b ? a.b[p.c0 + c] : 0.f;
+    const int g = p.on ? (p.c0 + c) / a.Cg : g0;
+    const float* st = a.stats + (sample_of(a) * a.G + g) * 2;
+    mean[c] = st[0];
+    rstd[c] = st[1];
+    if (DX) { s1[c] = lds[2 * (g - g0)]; s2[c] = lds[2 * (g - g0) + 1]; }
+    s[0][c] = s[1][c] = 0.f;
+  }
+  const int64_t base = sample_of(a) * a.S * a.C + p.c0;
+  const IO* x = reinterpret_cast<const IO*>(a.x) + base;
+  const IO* dy = reinterpret_cast<const IO*>(a.dy) + base;
+  IO* dx = reinterpret_cast<IO*>(a.y) + base;
+  auto one = [&](float (&v)[VEC], float (&d)[VEC], int64_t r) {
+    float z[VEC];
+#pragma unroll
+    for (int c = 0; c < VEC; ++c) {
+      v[c] = (v[c] - mean[c]) * rstd[c];
+      z[c] = fmaf(w[c], v[c], b[c]);
+    }
+    slope<VEC>(d, z, a.act);
+    if (!DX) {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) { s[0][c] = fmaf(d[c], v[c], s[0][c]); s[1][c] += d[c]; }
+    } else {
+#pragma unroll
+      for (int c = 0; c < VEC; ++c) d[c] = rstd[c] * (w[c] * d[c] - s1[c] - v[c] * s2[c]);
+      put<IO, VEC>(dx + r * a.C, d);
+    }
+  };
+  if (p.on) {
+    int64_t r = p.r0 + p.tr;
+    for (; r + p.rp < p.r1; r += 2 * p.rp) {
+      float v0[VEC], v1[VEC], d0[VEC], d1[VEC];
+      get<IO, VEC>(x + r * a.C, v0);
+      get<IO, VEC>(dy + r * a.C, d0);
+      get<IO, VEC>(x + (r + p.rp) * a.C, v1);
+      get<IO, VEC>(dy + (r + p.rp) * a.C, d1);
+      one(v0, d0, r);
+      one(v1, d1, r + p.rp);
+    }
+    for (; r < p.r1; r += p.rp) {
+      float v0[VEC], d0[VEC];
+      get<IO, VEC>(x + r * a.C, v0);
+      get<IO, VEC>(dy + r * a.C, d0);
+      one(v0, d0, r);
+    }
+  }
+  if (!DX) slice_sums<VEC>(a, p, s, lds);
+}
+
+// dw[c], db[c]: the sums of n partial rows ws[i][2][C], sixteen runs of rows a channel joined in order
+__global__ __launch_bounds__(256) void norm_params_kernel(const float* ws, int64_t n, int C, float* dw, float* db) {
+  __shared__ float part[16][16];
+  const int q = (int)blockIdx.y, cc = (int)threadIdx.x & 15, run = (int)threadIdx.x >> 4;
+  const int c = (int)blockIdx.x * 16 + cc;
+  float t = 0.f;
+  if (c < C) {
+    const float* p = ws + (int64_t)q * C + c;
+    int64_t i = run;
+    for (; i + 7 * 16 < n; i += 8 * 16) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = p[(i + 16 * u) * 2 * C];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t += v[u];
+    }
+    for (; i < n; i += 16) t += p[i * 2 * C];
+  }
+  part[run][cc] = t;
+  __syncthreads();
+  float* out = q == 0 ? dw : db;
+  if (run == 0 && c < C && out) {
+    float s = 0.f;
+    for (int r = 0; r < 16; ++r) s += part[r][cc];
+    out[c] = s;
+  }
+}
+
+struct Plan { bool rows; int vec, nv, lanes, groups_y, reps, grid_x, grid_y, slices, grid_z; int64_t slice_rows, parts; };
+
+Plan plan(int64_t B, int64_t S, int64_t C, int64_t G, int dtype, bool aligned) {
+  Plan p;
+  const int64_t Cg = C / G;
+  const int widest = dtype == PGT_DT_F32 ? 4 : 8;
+  p.vec = aligned ? widest : 1;
+  while (p.vec > 1 && Cg % p.vec) p.vec >>= 1;
+  const int64_t vecs = Cg / p.vec;
+  p.rows = S == 1 && vecs <= 64 * 8;
+  p.slices = p.grid_z = 1;
+  p.slice_rows = S;
+  if (p.rows) {
+    p.lanes = 1;
+    while (p.lanes < 64 && p.lanes < vecs) p.lanes <<= 1;
+    const int64_t nv = pgt_cdiv(vecs, p.lanes);
+    p.nv = nv <= 1 ? 1 : nv <= 2 ? 2 : nv <= 4 ? 4 : 8;
+    const int cl = 256 / p.lanes;
+    p.groups_y = (int)(G < cl ? G : cl);
+    p.reps = cl / p.groups_y;
+    p.grid_y = (int)pgt_cdiv(G, p.groups_y);
+    const int64_t want = pgt_cdiv(B, p.reps), most = pgt_cdiv(2048, p.grid_y);
+    p.grid_x = (int)(want < most ? want : most);
+    p.parts = p.grid_x;
+    return p;
+  }
+  p.vec = aligned ? widest : 1;
+  while (p.vec > 1 && C % p.vec) p.vec >>= 1;
+  const int64_t nq = C / p.vec;
+  p.grid_z = (int)pgt_cdiv(nq, 256);
+  const int64_t rp = nq >= 256 ? 1 : 256 / nq;
+  // about 1024 workgroups, slices of at least four passes over rows: a slice's sums are joined by every workgroup of the sample
+  int64_t slices = pgt_cdiv(1024, B * p.grid_z);
+  const int64_t by_rows = pgt_cdiv(S, 4 * rp);
+  if (slices > by_rows) slices = by_rows;
+  if (slices > 64) slices = 64;
+  if (slices < 1) slices = 1;
+  p.slice_rows = pgt_cdiv(pgt_cdiv(S, slices), rp) * rp;
+  p.slices = (int)pgt_cdiv(S, p.slice_rows);
+  p.parts = B * p.slices;
+  return p;
+}
+
+int check(const char* who, int64_t B, int64_t S, int64_t C, int64_t G, int dtype, int act) {
+  PGT_REQUIRE(dtype == PGT_DT_F32 || dtype == PGT_DT_BF16 || dtype == PGT_DT_F16, "%s: unknown dtype %d", who, dtype);
+  PGT_REQUIRE(act == PGT_ACT_NONE || act == PGT_ACT_RELU || act == PGT_ACT_SILU, "%s: unknown activation %d", who, act);
+  PGT_REQUIRE(B >= 0 && S >= 0 && C >= 1 && G >= 1 && C % G == 0, "%s: %lld channels do not divide into %lld groups", who, (long long)C, (long long)G);
+  PGT_REQUIRE(C <= (1 << 20) && S < ((int64_t)1 << 40) && B < ((int64_t)1 << 40), "%s: size out of range (at most 2^20 channels)", who);
+  return PGT_OK;
+}
+void fill(NormArgs& a, const Plan& p, int64_t B, int64_t S, int64_t C, int64_t G, float eps, int act) {
+  a.B = B; a.S = S; a.C = (int)C; a.G = (int)G; a.Cg = (int)(C / G); a.act = act; a.eps = eps;
+  a.slices = p.slices; a.lanes = p.lanes; a.groups_y = p.groups_y; a.reps = p.reps; a.slice_rows = p.slice_rows;
+}
+
+template <class IO, int VEC, bool BWD> void go_rows(const NormArgs& a, const Plan& p, pgt_stream_t stream) {
+  const dim3 grid((unsigned)p.grid_x, (unsigned)p.grid_y);
+  if (p.nv == 1) PGT_LAUNCH((norm_rows_kernel<IO, VEC, 1, BWD>), grid, dim3(256), stream, a);
+  else if (p.nv == 2) PGT_LAUNCH((norm_rows_kernel<IO, VEC, 2, BWD>), grid, dim3(256), stream, a);
+  else if (p.nv == 4) PGT_LAUNCH((norm_rows_kernel<IO, VEC, 4, BWD>), grid, dim3(256), stream, a);
+  else PGT_LAUNCH((norm_rows_kernel<IO, VEC, 8, BWD>), grid, dim3(256), stream, a);
+}
+template <class IO, int VEC> void go(const NormArgs& a, const Plan& p, bool bwd, pgt_stream_t stream) {
+  if (p.rows) {
+    if (bwd) go_rows<IO, VEC, true>(a, p, stream); else go_rows<IO, VEC, false>(a, p, stream);
+    return;
+  }
+  NormArgs l = a;
+  for (l.b0 = 0; l.b0 < a.B; l.b0 += 32768) {             // a grid's second axis ends at 65535
+    const dim3 grid((unsigned)p.slices, (unsigned)(a.B - l.b0 < 32768 ? a.B - l.b0 : 32768), (unsigned)p.grid_z);
+    if (!bwd) {
+      PGT_LAUNCH((norm_stats_kernel<IO, VEC>), grid, dim3(256), stream, l);
+      PGT_LAUNCH((norm_apply_kernel<IO, VEC>), grid, dim3(256), stream, l);
+    } else {
+      PGT_LAUNCH((norm_bwd_kernel<IO, VEC, false>), grid, dim3(256), stream, l);
+      if (a.y) PGT_LAUNCH((norm_bwd_kernel<IO, VEC, true>), grid, dim3(256), stream, l);
+    }
+  }
+}
+template <class IO> void by_vec(const NormArgs& a, const Plan& p, bool bwd, pgt_stream_t stream) {
+  if constexpr (sizeof(IO) == 2)
+    if (p.vec == 8) { go<IO, 8>(a, p, bwd, stream); return; }
+  if (p.vec == 4) go<IO, 4>(a, p, bwd, stream);
+  else if (p.vec == 2) go<IO, 2>(a, p, bwd, stream);
+  else go<IO, 1>(a, p, bwd, stream);
+}
+void by_type(const NormArgs& a, const Plan& p, int dtype, bool bwd, pgt_stream_t stream) {
+  if (dtype == PGT_DT_F32) by_vec<float>(a, p, bwd, stream);
+  else if (dtype == PGT_DT_BF16) by_vec<bf16>(a, p, bwd, stream);
+  else by_vec<f16>(a, p, bwd, stream);
+}
+
+}  // namespace
+
+extern "C" int64_t pgt_group_norm_ws_floats(int64_t batch, int64_t rows, int64_t channels, int64_t groups, int dtype, int adjoint) {
+  if (check("pgt_group_norm_ws_floats", batch, rows, channels, groups, dtype, 0)) return -1;
+  if (batch == 0 || rows == 0) return 0;
+  int64_t most = 0;
+  for (int al = 0; al < 2; ++al) {                         // whatever the tensors' alignment
+    const Plan p = plan(batch, rows, channels, groups, dtype, al != 0);
+    const int64_t n = p.rows && !adjoint ? 0 : p.parts * 2 * channels;
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+extern "C" int pgt_group_norm_act(const void* x, int64_t batch, int64_t rows, int64_t channels, int64_t groups, int dtype,
+                                  const float* weight, const float* bias, float eps, int act, void* y, float* stats, float* ws,
+                                  int64_t ws_floats, pgt_stream_t stream) {
+  const char* who = "pgt_group_norm_act";
+  if (int e = check(who, batch, rows, channels, groups, dtype, act)) return e;
+  if (batch == 0 || rows == 0) return PGT_OK;
+  PGT_REQUIRE(x && y, "%s: null pointer", who);
+  const Plan p = plan(batch, rows, channels, groups, dtype, pgt_aligned(x, 16) && pgt_aligned(y, 16));
+  if (!p.rows && (!ws || ws_floats < p.parts * 2 * channels)) {
+    pgt_set_error("%s: ws of %lld floats needed", who, (long long)(p.parts * 2 * channels));
+    return PGT_ERR_WORKSPACE;
+  }
+  NormArgs a = {};
+  fill(a, p, batch, rows, channels, groups, eps, act);
+  a.x = x; a.y = y; a.w = weight; a.b = bias; a.stats = stats; a.ws = ws;
+  by_type(a, p, dtype, false, stream);
+  return pgt_check_launch(who);
+}
+
+extern "C" int pgt_group_norm_act_bwd(const void* x, const void* dy, const float* stats, int64_t batch, int64_t rows, int64_t channels,
+                                      int64_t groups, int dtype, const float* weight, const float* bias, float eps, int act, void* dx,
+                                      float* dweight, float* dbias, float* ws, int64_t ws_floats, pgt_stream_t stream) {
+  const char* who = "pgt_group_norm_act_bwd";
+  if (int e = check(who, batch, rows, channels, groups, dtype, act)) return e;
+  if (batch == 0 || rows == 0) {                           // sums of nothing: a launch of no partial rows writes the zeros
+    if (dweight || dbias)
+      PGT_LAUNCH(norm_params_kernel, dim3((unsigned)pgt_cdiv(channels, 16), 2), dim3(256), stream, (const float*)nullptr, (int64_t)0, (int)channels, dweight, dbias);
+    return pgt_check_launch(who);
+  }
+  PGT_REQUIRE(x && dy, "%s: null pointer", who);
+  const Plan p = plan(batch, rows, channels, groups, dtype, pgt_aligned(x, 16) && pgt_aligned(dy, 16) && pgt_aligned(dx, 16));
+  const bool params = dweight || dbias;
+  PGT_REQUIRE(p.rows || stats, "%s: stats of the forward pass are needed", who);
+  if (!params && p.rows) ws = nullptr;
+  else if (!ws || ws_floats < p.parts * 2 * channels) {
+    pgt_set_error("%s: ws of %lld floats needed", who, (long long)(p.parts * 2 * channels));
+    return PGT_ERR_WORKSPACE;
+  }
+  NormArgs a = {};
+  fill(a, p, batch, rows, channels, groups, eps, act);
+  a.x = x; a.dy = dy; a.y = dx; a.w = weight; a.b = bias; a.stats = const_cast<float*>(stats); a.ws = ws;
+  by_type(a, p, dtype, true, stream);
+  if (params) {
+    const dim3 grid((unsigned)pgt_cdiv(channels, 16), 2);
+    PGT_LAUNCH(norm_params_kernel, grid, dim3(256), stream, (const float*)ws, p.parts, (int)channels, dweight, dbias);
+  }
+  return pgt_check_launch(who);
+}

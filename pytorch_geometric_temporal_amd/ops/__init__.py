@@ -13,6 +13,7 @@ One module per model family (round 5 kept all of this in one 2 800-line file):
     evolve    EvolveGCN-H / -O weight evolution, the small-graph GCN layer
     stconv    STConv: TemporalConv, node-wise batch norm
     delta     gated delta rule: sequences and single steps
+    norm      group norm with an activation
     generic   aggregation / linear / read-out Functions shared by the families
 
 `ops.NAME` is the public spelling of every name below, as before.  The package is also where the SWITCHES are flipped
@@ -23,9 +24,9 @@ imported it — so the code that reads the switch sees it whichever module it li
 import sys
 import types
 
-from . import _graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv, delta
+from . import _graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv, delta, norm
 
-_FAMILIES = (_graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv, delta)
+_FAMILIES = (_graphs, _core, dcrnn, generic, tgcn, cheb, astgcn, evolve, stconv, delta, norm)
 
 for _m in _FAMILIES:
     for _k, _v in vars(_m).items():

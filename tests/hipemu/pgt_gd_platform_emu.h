@@ -31,6 +31,9 @@ template <int N> static inline double gd_shr16(double x) {          // lane i ta
   const double y = __shfl(x, (__lane_id() & 48) | ((__lane_id() - N) & 15));
   return (__lane_id() & 15) >= N ? y : 0.0;
 }
+static inline float gd_xsum(float x, int lanes) { for (int m = 1; m < lanes; m <<= 1) x += __shfl_xor(x, m); return x; }
+static inline float gd_rcp(float x) { return 1.f / x; }
+static inline float gd_exp(float x) { return expf(x); }
 static inline void gd_wave_sync() { pgt_emu::wave_barrier(); }
 static inline void gd_block_sync() { __syncthreads(); }
 static inline float gd_as_float(uint32_t u) { float f; memcpy(&f, &u, 4); return f; }
