@@ -32,22 +32,33 @@ struct BwdArgs {
   int vec, vec_do, vec_e, vec_s; // q, k / d_o / e / states can be read four values at a time
 };
 
-// One team per sequence and segment, chunks from the last to the first.  STATE: only the gradient of the state before the segment, from a
-// zero gradient behind it (the last segment: from d_last).
-template <class IO, int D, bool STATE>
-__global__ __launch_bounds__(Team<D>::THREADS) void delta_bwd_kernel(BwdArgs a) {
+// One team per sequence and segment, chunks from the last to the first.  A wavefront owns sixteen value columns of dS and, in the
+// products for dQ and dK, sixteen key columns.  A chunk in three parts, a barrier between:
+//   1  the tiles that do not depend on dS, a wavefront each: K K^T and (I + A)^-T; Q K^T, P; dO E^T, M1 (and the previous chunk's dg)
+//   2  by value columns: dU, dR, dY, the new dS; the old dS and dY go to LDS, dY E^T as partial sums
+//   3  by key columns: dQ, dK and the row sums of dbeta and dg
+// Tiles named [j][i] hold row j, column i of the transposed tile: an A operand of the transposed product read along rows, of the
+// product itself read down columns.  Bound by the fp32 matrix pipe from K = 64 on (2 K + 22 MFMAs of 32 cycles a wavefront and chunk).
+// STATE: only the gradient of the state before the segment, from a zero gradient behind it (the last segment: from d_last).
+// FULL: K = V = D and every row can be read four values at a time.
+template <class IO, int D, bool STATE, bool FULL>
+__global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_kernel(BwdArgs a) {
   using TM = Team<D>;
-  constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, EPL = TM::EPL, NP = STATE ? 2 : 3;
+  constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, NT = D / 16;
+  constexpr int W_KQ = NW > 1 ? 1 : 0, W_OE = NW > 2 ? 2 : NW - 1, W_DG = NW > 2 ? 3 : 0;     // who does what in part 1
   struct Lds {
-    float k[16 * LD], q[16 * LD], o[16 * LD], e[STATE ? 4 : 16 * LD], y[16 * LD];
-    float x[STATE ? 4 : D * LD];                           // dS, for the products that contract over its columns
-    float part[NW][NP][TILE];
-    float at[TILE], pm[TILE], m1[TILE], m2[TILE], xm[TILE];
-    float red[NW][4][16];                                  // row sums by wavefront: dbeta, z, w, <S0, dS>
-    float hi[16], lo[16], enter[16], leave[16], beta[16], whole[4];
+    float k[16 * LD], q[16 * LD], o[16 * LD], e[STATE ? 4 : 16 * LD], y[STATE ? 4 : 16 * LD];
+    float x[STATE ? 4 : D * LD];                           // dS, for the product that contracts over its columns
+    float inv[256], p[256];                                // A operands, four values a lane
+    float am[TILE], m1[STATE ? 4 : TILE];                  // [j][i]
+    float kk[STATE ? 4 : 256], qk[STATE ? 4 : 256], db[STATE ? 4 : 256];      // K K^T, Q K^T, D_ij beta_j (i > j), as [j][i] four values a lane
+    float ye[STATE ? 1 : NW][STATE ? 4 : TILE];            // dY E^T by wavefront, [j][i]
+    float red[STATE ? 1 : NW][4][16];                      // row sums by wavefront: dbeta, z, w, <S0, dS>
+    float hi[NW][16], lo[NW][16], enter[16], leave[16], beta[16], whole[4];
   };
   __shared__ __attribute__((aligned(16))) char smem[sizeof(Lds) * TM::TEAMS];
   const Shape& s = a.s;
+  const int K = FULL ? D : s.K, V = FULL ? D : s.V;
   const int tid = (int)threadIdx.x, team = tid / TL, tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane = tid & 63, col = lane & 15, cg = lane >> 4;
   Lds& L = reinterpret_cast<Lds*>(smem)[team];
   const int64_t first = s.p0 + (int64_t)blockIdx.x * TM::TEAMS;
@@ -56,148 +67,204 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_bwd_kernel(BwdArgs a) 
   const int c0 = seg * s.cps, c1 = c0 + s.cps < s.chunks ? c0 + s.cps : s.chunks;
   const int reach = chunks_of_block<TM::TEAMS>(s, first), ce = reach < c1 ? reach : c1;
   const int kh = sq.h / s.rep;
-  const IO* kp = at<IO>(a.k, sq, kh);
-  const IO* qp = at<IO>(a.q, sq, kh);
   const float* gp = at<float>(a.g, sq, sq.h);
   const float* bp = at<float>(a.beta, sq, sq.h);
-  const int n = 16 * w + col;                             // this lane's column: of the state (values) and, in the dQ / dK products, of the keys
-  const bool vcols = 16 * w < s.V, kcols = 16 * w < s.K;
+  const int n = 16 * w + col;                             // this lane's column: of the values in part 2, of the keys in part 3
+  const bool vcols = FULL || 16 * w < V, kcols = FULL || 16 * w < K, vin = FULL || n < V, kin = FULL || n < K;
   const int64_t row_h = (int64_t)s.N * s.H, seq_h = (int64_t)sq.b * s.T * row_h + (int64_t)sq.n * s.H + sq.h;     // rows of [B, T, N, H]
 
-  gd_f4 S[QD / 4];                                        // dS
+  gd_f4 S[NT];                                            // dS
   {
     const float* from = seg == s.segs - 1 ? a.d_last : STATE ? nullptr : a.seg_end;
-    if (from) from += seg == s.segs - 1 ? sq.p * s.K * s.V : (sq.p * (s.segs - 1) + seg) * s.K * s.V;
 #pragma unroll
-    for (int t = 0; t < QD / 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * t + 4 * cg + r;
-        S[t][r] = from && sq.live && row < s.K && n < s.V ? from[(int64_t)row * s.V + n] : 0.f;
-      }
+    for (int t = 0; t < NT; ++t) S[t] = zero4();
+    if (from && sq.live) load_state<NT, FULL>(S, from + (seg == s.segs - 1 ? sq.p : sq.p * (s.segs - 1) + seg) * K * V, K, V, n, cg);
   }
   const int tok = tl / QD, qd = 4 * (tl % QD);
-  gd_f4 nk = zero4(), nq = zero4(), no = zero4(), ne = zero4();
+  const IO* kp = at<IO>(a.k, sq, kh) + tok * a.k.st + qd;
+  const IO* qp = at<IO>(a.q, sq, kh) + tok * a.q.st + qd;
+  const int64_t row_v = row_h * V;
+  const IO* op = reinterpret_cast<const IO*>(a.d_o) + seq_h * V + tok * row_v + qd;
+  const float* ep = a.e + seq_h * V + tok * row_v + qd;
+  Quad<IO> nk, nq, no;
+  Quad<float> ne;
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
-    const int t = 16 * c + tok;
-    const bool in = t < sq.len;
-    nk = load4(kp + (int64_t)t * a.k.st + qd, in ? s.K - qd : 0, a.vec != 0);
-    nq = load4(qp + (int64_t)t * a.q.st + qd, in ? s.K - qd : 0, a.vec != 0);
-    const int64_t off = (seq_h + t * row_h) * s.V + qd;
-    no = load4(reinterpret_cast<const IO*>(a.d_o) + off, in ? s.V - qd : 0, a.vec_do != 0);
-    if (!STATE) ne = load4(a.e + off, in ? s.V - qd : 0, a.vec_e != 0);
-    if (w == 0) {
-      const int tg = 16 * c + col;
-      ng = tg < sq.len ? gp[(int64_t)tg * a.g.st] : 0.f;
-      nb = tg < sq.len ? bp[(int64_t)tg * a.beta.st] : 0.f;
+    const int64_t t0 = 16 * c;
+    const bool in = t0 + tok < sq.len;
+    read4<FULL>(nk, kp + t0 * a.k.st, in ? K - qd : 0, a.vec != 0);
+    read4<FULL>(nq, qp + t0 * a.q.st, in ? K - qd : 0, a.vec != 0);
+    read4<FULL>(no, op + t0 * row_v, in ? V - qd : 0, a.vec_do != 0);
+    if (!STATE) read4<FULL>(ne, ep + t0 * row_v, in ? V - qd : 0, a.vec_e != 0);
+    const int tg = 16 * c + col;
+    ng = nb = 0.f;
+    if (tg < sq.len) { ng = gp[tg * a.g.st]; nb = bp[tg * a.beta.st]; }
+  };
+  // dg and dbeta of chunk c, while the next one's tiles are made, from the row sums in LDS and
+  // X_ij = M1_ij q_i.k_j + M2_ij k_i.k_j left of the diagonal (row i = 4 cg + r, column j = col), which wavefront W_DG kept
+  gd_f4 pre = zero4();
+  auto finish = [&](int c) {
+    float dbv = 0.f, z = 0.f, wj = 0.f, dot = 0.f;
+#pragma unroll
+    for (int u = 0; u < NW; ++u) {
+      dbv += L.red[u][0][col];
+      z += L.red[u][1][col];
+      wj += L.red[u][2][col];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dot += L.red[u][3][i];
+    }
+    // c_l = sum_{i >= l} sum_{j < l} X_ij: for every l the lanes of columns j < l add their rows i >= l
+    gd_f4 suf;                                            // sum over rows i >= 4 cg + r of this lane's group of four
+    suf[3] = pre[3];
+    suf[2] = pre[2] + suf[3];
+    suf[1] = pre[1] + suf[2];
+    suf[0] = pre[0] + suf[1];
+    float above = 0.f;                                    // the groups of four behind this one
+    const float s1 = __shfl(suf[0], col + 16), s2 = __shfl(suf[0], col + 32), s3 = __shfl(suf[0], col + 48);
+    above = cg == 0 ? s1 + (s2 + s3) : cg == 1 ? s2 + s3 : cg == 2 ? s3 : 0.f;
+    const float whole = L.whole[0];
+    gd_f4 dg;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int l = 4 * cg + r;                           // column col adds its rows >= l where col < l; step col its z where col >= l, its w where not
+      dg[r] = sum16(col < l ? suf[r] + above + wj : z) + dot * whole;
+    }
+    const int64_t at = seq_h + (int64_t)(16 * c) * row_h;
+    if (sq.live && lane < 16 && 16 * c + lane < s.T) a.dbeta[at + lane * row_h] = 16 * c + lane < sq.len ? dbv : 0.f;
+    if (sq.live && col < 4) {
+      const int l = 4 * cg + col;
+      const float x = col == 0 ? dg[0] : col == 1 ? dg[1] : col == 2 ? dg[2] : dg[3];
+      if (16 * c + l < s.T) a.dg[at + l * row_h] = 16 * c + l < sq.len ? x : 0.f;
     }
   };
   if (c0 < ce) fetch(ce - 1);
   for (int c = ce - 1; c >= c0; --c) {
-    put4(&L.k[tok * LD + qd], nk);
+    put4(&L.k[tok * LD + qd], unpack(nk));
+    {
+      gd_f4 x = unpack(nq);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) nq[r] *= s.scale;
-    put4(&L.q[tok * LD + qd], nq);
-    put4(&L.o[tok * LD + qd], no);
-    if (!STATE) put4(&L.e[tok * LD + qd], ne);
-    if (w == 0) {
-      const Decay d = chunk_decay(ng);
-      if (lane < 16) {
-        L.hi[lane] = d.hi; L.lo[lane] = d.lo; L.enter[lane] = d.enter; L.leave[lane] = d.leave; L.beta[lane] = nb;
-        if (lane == 0) L.whole[0] = d.whole;
-      }
+      for (int r = 0; r < 4; ++r) x[r] *= s.scale;
+      put4(&L.q[tok * LD + qd], x);
     }
+    put4(&L.o[tok * LD + qd], unpack(no));
+    if (!STATE) put4(&L.e[tok * LD + qd], unpack(ne));
+    const float g = ng, b = nb;
     if (c > c0) fetch(c - 1);
-    gd_f4 s0[STATE ? 1 : QD / 4];                         // S0, rows = this wavefront's sixteen key columns, along the values
-    if (!STATE) {
-      const float* from = c > 0 ? a.states + (sq.p * (s.chunks - 1) + c - 1) * s.K * s.V : a.start ? a.start + sq.p * s.K * s.V : nullptr;
+    gd_f4 s0[STATE ? 1 : NT];                             // S0, row = this lane's key column, along the values
+    const float* from = c > 0 ? a.states + (sq.p * (s.chunks - 1) + c - 1) * K * V : a.start ? a.start + sq.p * K * V : nullptr;
+    if (!STATE) {                                         // (without a state any valid address: no branch around register arrays)
+      const float* base = from ? from : a.e;
+      const bool in = from && kin;
 #pragma unroll
-      for (int t = 0; t < QD / 4; ++t)
-        s0[t] = load4(from + (int64_t)n * s.V + 16 * t + 4 * cg, from && sq.live && n < s.K ? s.V - 16 * t - 4 * cg : 0, a.vec_s != 0);
-    }
-    team_sync<D>();
-    {   // this wavefront's sixteen columns of K K^T, Q K^T (keys) and dO U^T (values)
-      const gd_f4 kk = lds4(&L.k[col * LD + 16 * w + 4 * cg]);
-      const gd_f4 x = mma16(kk, kk, zero4()), y = mma16(lds4(&L.q[col * LD + 16 * w + 4 * cg]), kk, zero4());
-      gd_f4 z = zero4();
-      if (!STATE) {
-        gd_f4 u = lds4(&L.e[col * LD + 16 * w + 4 * cg]);
-        const float b = L.beta[col];
+      for (int t = 0; t < NT; ++t) {
+        const int at = 16 * t + 4 * cg, left = V - at;
+        if (FULL) {
+          s0[t] = lds4(base + (in ? n * V + at : 0));
+        } else if (a.vec_s) {
+          const gd_f4 x = lds4(base + (in && left > 0 ? n * V + at : 0));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) u[r] *= b;
-        z = mma16(lds4(&L.o[col * LD + 16 * w + 4 * cg]), u, z);
-      }
+          for (int r = 0; r < 4; ++r) s0[t][r] = in && left > 0 ? x[r] : 0.f;
+        } else {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        L.part[w][0][(4 * cg + r) * TS + col] = x[r];
-        L.part[w][1][(4 * cg + r) * TS + col] = y[r];
-        if (!STATE) L.part[w][NP - 1][(4 * cg + r) * TS + col] = z[r];
-      }
-    }
-    team_sync<D>();
-    float el_d[EPL], el_kd[EPL], el_x[EPL];
-    if (tl < 256) {
-#pragma unroll
-      for (int m = 0; m < EPL; ++m) {
-        const int el = tl + m * TL, i = el >> 4, j = el & 15;
-        float kk = 0.f, qk = 0.f, ou = 0.f;
-#pragma unroll
-        for (int u = 0; u < NW; ++u) {
-          kk += L.part[u][0][i * TS + j];
-          qk += L.part[u][1][i * TS + j];
-          if (!STATE) ou += L.part[u][NP - 1][i * TS + j];
+          for (int r = 0; r < 4; ++r) {
+            const float x = base[in && r < left ? n * V + at + r : 0];
+            s0[t][r] = in && r < left ? x : 0.f;
+          }
         }
-        const float d = j <= i ? expf((L.hi[i] - L.hi[j]) + (L.lo[i] - L.lo[j])) : 0.f;
-        L.at[j * TS + i] = j < i ? L.beta[i] * d * kk : 0.f;
-        L.pm[i * TS + j] = j <= i ? d * qk : 0.f;
+      }
+    }
+    team_sync<D>();
+    // ---- part 1
+    if (!STATE && w == W_DG && c < ce - 1) finish(c + 1);
+    if (w == 0 || w == W_KQ || (!STATE && w == W_OE)) {
+      const Decay d = chunk_decay(g);
+      if (lane < 16) { L.hi[w][lane] = d.hi; L.lo[w][lane] = d.lo; }
+      if (w == 0 && lane < 16) {
+        L.enter[lane] = d.enter; L.leave[lane] = d.leave; L.beta[lane] = b;
+      }
+      gd_f4 kk = zero4(), qk = zero4(), oe = zero4();     // row i = 4 cg + r, column j = col
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        gd_f4 x = zero4();
+        if (w == 0 || w == W_KQ) x = lds4(&L.k[col * LD + 16 * t + 4 * cg]);
+        if (w == 0) kk = mma16(x, x, kk);
+        if (w == W_KQ) qk = mma16(lds4(&L.q[col * LD + 16 * t + 4 * cg]), x, qk);
+        if (!STATE && w == W_OE) oe = mma16(lds4(&L.o[col * LD + 16 * t + 4 * cg]), lds4(&L.e[col * LD + 16 * t + 4 * cg]), oe);
+      }
+      gd_wave_sync();
+      const gd_f4 hi = lds4(&L.hi[w][4 * cg]), li = lds4(&L.lo[w][4 * cg]);
+      gd_f4 dec;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dec[r] = 4 * cg + r >= col ? gd_exp2((hi[r] - d.hi) + (li[r] - d.lo)) : 0.f;
+      if (w == W_KQ) {
+        gd_f4 p;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = dec[r] * qk[r];
+        put4(&L.p[4 * lane], p);
+        if (!STATE) put4(&L.qk[4 * lane], qk);
+      }
+      if (!STATE && w == W_OE) {
+        gd_f4 m;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          dec[r] *= b;
+          m[r] = dec[r] * oe[r];
+        }
+        put4(&L.m1[col * TS + 4 * cg], m);
+      }
+      if (w == 0) {
+        const gd_f4 bi = lds4(&L.beta[4 * cg]);
+        gd_f4 m, db;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = 4 * cg + r > col ? (NW > 2 || STATE ? dec[r] : gd_exp2((hi[r] - d.hi) + (li[r] - d.lo))) : 0.f;
+          m[r] = bi[r] * x * kk[r];
+          db[r] = x * b;
+        }
         if (!STATE) {
-          const float m1 = j <= i ? d * ou : 0.f;
-          L.m1[i * TS + j] = m1;
-          el_d[m] = j < i ? d : 0.f;
-          el_kd[m] = j < i ? d * kk : 0.f;
-          el_x[m] = j < i ? m1 * qk : 0.f;
+          put4(&L.kk[4 * lane], kk);
+          put4(&L.db[4 * lane], db);
         }
+        put4(&L.am[col * TS + 4 * cg], m);                // row j of A^T
+        gd_wave_sync();
+        float arow[16];
+        row16(&L.am[col * TS], arow);
+        gd_f4 inv = unit_row(lane);
+        solve_up<15>(arow, inv);
+        put4(&L.inv[4 * lane], inv);
       }
     }
     team_sync<D>();
+    // ---- part 2
     const gd_f4 enter = lds4(&L.enter[4 * cg]), leave = lds4(&L.leave[4 * cg]), beta = lds4(&L.beta[4 * cg]);
-    gd_f4 dy = zero4();
+    const float whole = L.enter[15];
+    if (w == 0 && lane == 0) L.whole[0] = whole;
     if (vcols) {
-      gd_f4 ks = zero4();
+      gd_f4 du = zero4();
 #pragma unroll
-      for (int t = 0; t < QD / 4; ++t) ks = mma16(lds4(&L.k[col * LD + 16 * t + 4 * cg]), S[t], ks);
-      gd_f4 dout, pt;
+      for (int t = 0; t < NT; ++t) {
+        if (t % 4 == 0) PGT_SCHED_FENCE();
+        du = mma16(lds4(&L.k[col * LD + 16 * t + 4 * cg]), S[t], du);
+      }
+      gd_f4 dout;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         dout[r] = L.o[(4 * cg + r) * LD + n];
-        pt[r] = L.pm[(4 * cg + r) * TS + col];
-        ks[r] *= leave[r];
+        du[r] *= leave[r];
       }
-      const gd_f4 du = mma16(pt, dout, ks);
-      float arow[16];
-      row16(&L.at[col * TS], arow);
-      gd_f4 inv = unit_row(lane);
-      solve_up<15>(arow, inv);
-      const gd_f4 dr = mma16(inv, du, zero4());
-      float db[4];
+      du = mma16(lds4(&L.p[4 * lane]), dout, du);
+      const gd_f4 dr = mma16(lds4(&L.inv[4 * lane]), du, zero4());
+      gd_f4 dy, eo, ey;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         dy[r] = beta[r] * dr[r];
-        if (!STATE) {
-          L.y[(4 * cg + r) * LD + n] = dy[r];
-          db[r] = sum16(dr[r] * L.e[(4 * cg + r) * LD + n]);
-          if (col == 0) L.red[w][0][4 * cg + r] = db[r];
-          const int t = 16 * c + 4 * cg + r;
-          if (sq.live && t < s.T && n < s.V) reinterpret_cast<IO*>(a.dv)[(seq_h + t * row_h) * s.V + n] = from_f32<IO>(dy[r]);
-        }
+        if (!STATE) L.y[(4 * cg + r) * LD + n] = dy[r];
+        eo[r] = enter[r] * dout[r];
+        ey[r] = -(enter[r] * dy[r]);
       }
-      const float whole = L.whole[0];
-      gd_f4 eo, ey;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) { eo[r] = enter[r] * dout[r]; ey[r] = -(enter[r] * dy[r]); }
-#pragma unroll
-      for (int t = 0; t < QD / 4; ++t) {
+      for (int t = 0; t < NT; ++t) {
+        if (t % 4 == 0) PGT_SCHED_FENCE();
         gd_f4 kt, qt;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -208,6 +275,22 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_bwd_kernel(BwdArgs a) 
         }
         S[t] = mma16(kt, ey, mma16(qt, eo, S[t]));
       }
+      if (!STATE) {
+        float db[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) db[r] = sum16(dr[r] * L.e[(4 * cg + r) * LD + n]);
+        if (col == 0) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) L.red[w][0][4 * cg + r] = db[r];
+        }
+        if (sq.live && vin) {
+          const int64_t at = (seq_h + (int64_t)(16 * c + 4 * cg) * row_h) * V + n;
+          const int left = s.T - 16 * c - 4 * cg;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < left) reinterpret_cast<IO*>(a.dv)[at + r * row_v] = from_f32<IO>(dy[r]);
+        }
+      }
     } else if (!STATE) {                                  // columns behind the values' width: the products below read them
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -215,61 +298,78 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_bwd_kernel(BwdArgs a) 
         if (col == 0) L.red[w][0][4 * cg + r] = 0.f;
       }
 #pragma unroll
-      for (int t = 0; t < QD / 4; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) L.x[(16 * t + 4 * cg + r) * LD + n] = 0.f;
     }
     if (!STATE) {
-      gd_wave_sync();
-      {   // dY U^T over this wavefront's sixteen value columns
-        gd_f4 u = lds4(&L.e[col * LD + 16 * w + 4 * cg]);
-        const float b = L.beta[col];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) u[r] *= b;
-        const gd_f4 z = mma16(lds4(&L.y[col * LD + 16 * w + 4 * cg]), u, zero4());
-#pragma unroll
-        for (int r = 0; r < 4; ++r) L.part[w][0][(4 * cg + r) * TS + col] = z[r];
-      }
+      gd_wave_sync();                                     // dY E^T over this wavefront's sixteen value columns
+      const gd_f4 z = mma16(lds4(&L.y[col * LD + 16 * w + 4 * cg]), lds4(&L.e[col * LD + 16 * w + 4 * cg]), zero4());
+      put4(&L.ye[w][col * TS + 4 * cg], z);
       team_sync<D>();
-      if (tl < 256) {
+      // ---- part 3
+      if (w == W_DG) {
+        const gd_f4 b = lds4(&L.db[4 * lane]), qk = lds4(&L.qk[4 * lane]), kk = lds4(&L.kk[4 * lane]), m1 = lds4(&L.m1[col * TS + 4 * cg]);
+        gd_f4 ye = zero4();
 #pragma unroll
-        for (int m = 0; m < EPL; ++m) {
-          const int el = tl + m * TL, i = el >> 4, j = el & 15;
-          float yu = 0.f;
+        for (int u = 0; u < NW; ++u) {
+          const gd_f4 y = lds4(&L.ye[u][col * TS + 4 * cg]);
 #pragma unroll
-          for (int u = 0; u < NW; ++u) yu += L.part[u][0][i * TS + j];
-          L.m2[i * TS + j] = -(yu * el_d[m]);
-          L.xm[i * TS + j] = el_x[m] - yu * el_kd[m];
+          for (int r = 0; r < 4; ++r) ye[r] += y[r];
         }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) pre[r] = 4 * cg + r > col ? m1[r] * qk[r] - b[r] * kk[r] * ye[r] : 0.f;
       }
-      team_sync<D>();
       if (kcols) {
         gd_f4 aq = zero4(), ak = zero4(), al = zero4();
         float dot = 0.f;
+        if (from) {
 #pragma unroll
-        for (int t = 0; t < QD / 4; ++t) {
-          aq = mma16(lds4(&L.o[col * LD + 16 * t + 4 * cg]), s0[t], aq);
-          ak = mma16(lds4(&L.y[col * LD + 16 * t + 4 * cg]), s0[t], ak);
-          const gd_f4 x = lds4(&L.x[n * LD + 16 * t + 4 * cg]);
-          gd_f4 u = lds4(&L.e[col * LD + 16 * t + 4 * cg]);
-          const float b = L.beta[col];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) { u[r] *= b; dot = fmaf(s0[t][r], x[r], dot); }
-          al = mma16(u, x, al);
+          for (int t = 0; t < NT; ++t) {
+            if (t % 4 == 0) PGT_SCHED_FENCE();
+            aq = mma16(lds4(&L.o[col * LD + 16 * t + 4 * cg]), s0[t], aq);
+            ak = mma16(lds4(&L.y[col * LD + 16 * t + 4 * cg]), s0[t], ak);
+          }
         }
-        gd_f4 kc, qc, m1 = lds4(&L.m1[col * TS + 4 * cg]), m1t, m2 = lds4(&L.m2[col * TS + 4 * cg]);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (t % 4 == 0) PGT_SCHED_FENCE();
+          const gd_f4 x = lds4(&L.x[n * LD + 16 * t + 4 * cg]);
+          if (from) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dot = fmaf(s0[t][r], x[r], dot);
+          }
+          al = mma16(lds4(&L.e[col * LD + 16 * t + 4 * cg]), x, al);
+        }
+        PGT_SCHED_FENCE();
+        // M2, as an A operand of its own and of its transpose
+        gd_f4 m2 = zero4(), m2t = zero4();
+#pragma unroll
+        for (int u = 0; u < NW; ++u) {
+          const gd_f4 y = lds4(&L.ye[u][col * TS + 4 * cg]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            m2t[r] += y[r];
+            m2[r] += L.ye[u][(4 * cg + r) * TS + col];
+          }
+        }
+        const gd_f4 bt = lds4(&L.db[4 * lane]);
+        const gd_f4 m1t = lds4(&L.m1[col * TS + 4 * cg]);
+        gd_f4 kc, qc, m1;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           kc[r] = L.k[(4 * cg + r) * LD + n];
           qc[r] = L.q[(4 * cg + r) * LD + n];
-          m1t[r] = L.m1[(4 * cg + r) * TS + col];
-          m2[r] += L.m2[(4 * cg + r) * TS + col];
+          m1[r] = L.m1[(4 * cg + r) * TS + col];
+          // the entry (i = 4 cg + r, j = col) of D beta lies with lane 16 (i / 4) + j as value i % 4: as written for this lane; its mirror
+          // (i = col, j = 4 cg + r) with lane 16 (col / 4) + 4 cg + r as value col % 4
+          m2[r] = -(m2[r] * L.db[4 * (16 * (col >> 2) + 4 * cg + r) + (col & 3)]) - m2t[r] * bt[r];
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           aq[r] *= enter[r];
           ak[r] *= -enter[r];
-          al[r] *= leave[r];
+          al[r] *= leave[r] * beta[r];
           const float z = sum16(qc[r] * aq[r] + kc[r] * ak[r]), wj = sum16(kc[r] * al[r]);
           if (col == 0) { L.red[w][1][4 * cg + r] = z; L.red[w][2][4 * cg + r] = wj; }
           ak[r] += al[r];
@@ -279,18 +379,19 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_bwd_kernel(BwdArgs a) 
         aq = mma16(m1, kc, aq);
         ak = mma16(m2, kc, ak);
         ak = mma16(m1t, qc, ak);
-        if (sq.live && n < s.K) {
+        if (sq.live && kin) {
+          const int left = s.T - 16 * c - 4 * cg;
+          const int64_t row_k = (s.rep > 1 ? row_h : (int64_t)s.N * (s.H / s.rep)) * K;
+          const int64_t at = (s.rep > 1 ? seq_h : ((int64_t)sq.b * s.T * s.N + sq.n) * (s.H / s.rep) + kh) * K + (int64_t)(16 * c + 4 * cg) * row_k + n;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const int t = 16 * c + 4 * cg + r;
-            if (t < s.T) {
-              const int64_t off = (s.rep > 1 ? seq_h + t * row_h : (((int64_t)sq.b * s.T + t) * s.N + sq.n) * s.H + kh) * s.K + n;
+            if (r < left) {
               if (s.rep > 1) {
-                reinterpret_cast<float*>(a.dq)[off] = aq[r] * s.scale;
-                reinterpret_cast<float*>(a.dk)[off] = ak[r];
+                reinterpret_cast<float*>(a.dq)[at + r * row_k] = aq[r] * s.scale;
+                reinterpret_cast<float*>(a.dk)[at + r * row_k] = ak[r];
               } else {
-                reinterpret_cast<IO*>(a.dq)[off] = from_f32<IO>(aq[r] * s.scale);
-                reinterpret_cast<IO*>(a.dk)[off] = from_f32<IO>(ak[r]);
+                reinterpret_cast<IO*>(a.dq)[at + r * row_k] = from_f32<IO>(aq[r] * s.scale);
+                reinterpret_cast<IO*>(a.dk)[at + r * row_k] = from_f32<IO>(ak[r]);
               }
             }
           }
@@ -300,67 +401,27 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_bwd_kernel(BwdArgs a) 
         L.red[w][2][lane] = 0.f;
         L.red[w][3][lane] = 0.f;
       }
-      team_sync<D>();
-      if (w == 0) {
-        // lane l (of the first sixteen): dbeta_l; dg_l = c_l + sum_{i >= l} z_i + sum_{j < l} w_j + whole <S0, dS>
-        float db = 0.f, z = 0.f, wj = 0.f, dot = 0.f;
-#pragma unroll
-        for (int u = 0; u < NW; ++u) {
-          db += L.red[u][0][col];
-          z += L.red[u][1][col];
-          wj += L.red[u][2][col];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dot += L.red[u][3][i];
-        }
-        float dg = dot * L.whole[0];
-        for (int i = 0; i < 16; ++i) {
-          const float zi = __shfl(z, i, 16), wi = __shfl(wj, i, 16);
-          dg += i >= col ? zi : wi;
-        }
-        float c_l = 0.f;                                  // the tile's entries left of column l in the rows from l on
-        for (int i = 1; i < 16; ++i)
-          for (int jj = 0; jj < 4; ++jj) {
-            const int j = 4 * cg + jj;
-            c_l += i >= col && j < col ? L.xm[i * TS + j] : 0.f;
-          }
-        c_l += __shfl_xor(c_l, 16);
-        c_l += __shfl_xor(c_l, 32);
-        dg += c_l;
-        const int t = 16 * c + col;
-        if (sq.live && cg == 0 && t < s.T) {
-          a.dbeta[seq_h + t * row_h] = t < sq.len ? db : 0.f;
-          a.dg[seq_h + t * row_h] = t < sq.len ? dg : 0.f;
-        }
-      }
-    } else {
-      team_sync<D>();
     }
+    team_sync<D>();
   }
+  if (!STATE && w == W_DG && c0 < ce) finish(c0);
 
   if (sq.live) {
-    float* to = STATE ? a.seg_end + (sq.p * (s.segs - 1) + seg - 1) * s.K * s.V : seg == 0 && a.d_start ? a.d_start + sq.p * s.K * s.V : nullptr;
-    if (to) {
-#pragma unroll
-      for (int t = 0; t < QD / 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * t + 4 * cg + r;
-          if (row < s.K && n < s.V) to[(int64_t)row * s.V + n] = S[t][r];
-        }
-    }
+    float* to = STATE ? a.seg_end + (sq.p * (s.segs - 1) + seg - 1) * K * V : seg == 0 && a.d_start ? a.d_start + sq.p * K * V : nullptr;
+    if (to) store_state<NT, FULL>(S, to, K, V, n, cg);
     if (!STATE) {                                         // rows behind the sequence: zero
       const int lo = 16 * (ce > c0 ? ce : c0), hi = 16 * c1 < s.T ? 16 * c1 : s.T;
       for (int t = lo + tok; t < hi; t += 16) {
-        const int64_t row = seq_h + t * row_h, krow = s.rep > 1 ? row : (((int64_t)sq.b * s.T + t) * s.N + sq.n) * s.H + kh;
+        const int64_t row = seq_h + t * row_h, krow = s.rep > 1 ? row : (((int64_t)sq.b * s.T + t) * s.N + sq.n) * (s.H / s.rep) + kh;
         for (int r = 0; r < 4; ++r) {
-          if (qd + r < s.V) reinterpret_cast<IO*>(a.dv)[row * s.V + qd + r] = from_f32<IO>(0.f);
-          if (qd + r < s.K) {
+          if (qd + r < V) reinterpret_cast<IO*>(a.dv)[row * V + qd + r] = from_f32<IO>(0.f);
+          if (qd + r < K) {
             if (s.rep > 1) {
-              reinterpret_cast<float*>(a.dq)[krow * s.K + qd + r] = 0.f;
-              reinterpret_cast<float*>(a.dk)[krow * s.K + qd + r] = 0.f;
+              reinterpret_cast<float*>(a.dq)[krow * K + qd + r] = 0.f;
+              reinterpret_cast<float*>(a.dk)[krow * K + qd + r] = 0.f;
             } else {
-              reinterpret_cast<IO*>(a.dq)[krow * s.K + qd + r] = from_f32<IO>(0.f);
-              reinterpret_cast<IO*>(a.dk)[krow * s.K + qd + r] = from_f32<IO>(0.f);
+              reinterpret_cast<IO*>(a.dq)[krow * K + qd + r] = from_f32<IO>(0.f);
+              reinterpret_cast<IO*>(a.dk)[krow * K + qd + r] = from_f32<IO>(0.f);
             }
           }
         }
@@ -382,7 +443,7 @@ __global__ __launch_bounds__(256) void delta_heads_kernel(const float* x, IO* y,
   y[i] = from_f32<IO>(acc);
 }
 
-template <class IO, int D, bool STATE> void go(const BwdArgs& a0, pgt_stream_t stream) {
+template <class IO, int D, bool STATE, bool FULL> void go(const BwdArgs& a0, pgt_stream_t stream) {
   using TM = Team<D>;
   BwdArgs a = a0;
   const int64_t most = (int64_t)1 << 21;
@@ -390,16 +451,17 @@ template <class IO, int D, bool STATE> void go(const BwdArgs& a0, pgt_stream_t s
     a.s.p0 = p0;
     const int64_t wgs = pgt_cdiv(a.s.P - p0, TM::TEAMS);
     const dim3 grid((unsigned)(wgs < most ? wgs : most), (unsigned)(STATE ? a.s.segs - 1 : a.s.segs));
-    PGT_LAUNCH((delta_bwd_kernel<IO, D, STATE>), grid, dim3(TM::THREADS), stream, a);
+    PGT_LAUNCH((delta_bwd_kernel<IO, D, STATE, FULL>), grid, dim3(TM::THREADS), stream, a);
   }
 }
 template <class IO, int D> int all(const BwdArgs& a, const float* seg_trans, pgt_stream_t stream) {
+  const bool full = a.vec && a.vec_do && a.vec_e && a.vec_s && a.s.K == D && a.s.V == D;
   if (a.s.segs > 1) {
-    go<IO, D, true>(a, stream);
+    if (full) go<IO, D, true, true>(a, stream); else go<IO, D, true, false>(a, stream);
     if (a.s.segs > 2)
       if (int e = pgt_delta_join_up(seg_trans, a.seg_end, a.s.P, a.s.segs, a.s.K, a.s.V, stream)) return e;
   }
-  go<IO, D, false>(a, stream);
+  if (full) go<IO, D, false, true>(a, stream); else go<IO, D, false, false>(a, stream);
   return pgt_check_launch("pgt_gated_delta_bwd");
 }
 template <class IO> int by_width(const BwdArgs& a0, void* dq, void* dk, const float* seg_trans, pgt_stream_t stream) {
@@ -448,7 +510,7 @@ extern "C" int pgt_gated_delta_bwd(const pgt_delta_dims* d, const pgt_seq_view* 
   a.dv = dv; a.dg = dg; a.dbeta = dbeta; a.d_start = d_start; a.seg_end = seg_end;
   a.vec_do = a.s.V % 4 == 0 && pgt_aligned(d_o, d->dtype == PGT_DT_F32 ? 16 : 8);
   a.vec_e = a.s.V % 4 == 0 && pgt_aligned(e, 16);
-  a.vec_s = a.s.V % 4 == 0 && pgt_aligned(states, 16) && pgt_aligned(start, 16);
+  a.vec_s = a.vec_e && pgt_aligned(states, 16) && pgt_aligned(start, 16);
   if (d->dtype == PGT_DT_F32) return by_width<float>(a, dq, dk, seg_trans, stream);
   if (d->dtype == PGT_DT_BF16) return by_width<bf16>(a, dq, dk, seg_trans, stream);
   return by_width<f16>(a, dq, dk, seg_trans, stream);

@@ -46,6 +46,7 @@ __device__ __forceinline__ float gd_xsum(float x, int lanes) {
   if (lanes > 32) x += __shfl_xor(x, 32);
   return x;
 }
+__device__ __forceinline__ float gd_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float gd_rcp(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ __forceinline__ float gd_exp(float x) { return __expf(x); }
 // LDS hand-off inside one wavefront / inside the workgroup (global loads and stores stay in flight across it)
@@ -77,23 +78,6 @@ __device__ __forceinline__ gd_f4 load4(const float* p, int n, bool vec) {
   if (n > 1) r[1] = p[1];
   if (n > 2) r[2] = p[2];
   if (n > 3) r[3] = p[3];
-  return r;
-}
-template <class IO> __device__ __forceinline__ gd_f4 load4(const IO* p, int n, bool vec) {
-  gd_f4 r;
-  r[0] = r[1] = r[2] = r[3] = 0.f;
-  if (vec) {
-    if (n >= 4) {
-      const int2 t = *reinterpret_cast<const int2*>(p);
-      r[0] = to_f32(IO{(uint16_t)((uint32_t)t.x & 0xffffu)}); r[1] = to_f32(IO{(uint16_t)((uint32_t)t.x >> 16)});
-      r[2] = to_f32(IO{(uint16_t)((uint32_t)t.y & 0xffffu)}); r[3] = to_f32(IO{(uint16_t)((uint32_t)t.y >> 16)});
-    }
-    return r;
-  }
-  if (n > 0) r[0] = to_f32(p[0]);
-  if (n > 1) r[1] = to_f32(p[1]);
-  if (n > 2) r[2] = to_f32(p[2]);
-  if (n > 3) r[3] = to_f32(p[3]);
   return r;
 }
 __device__ __forceinline__ gd_f4 zero4() { gd_f4 r; r[0] = r[1] = r[2] = r[3] = 0.f; return r; }
@@ -149,13 +133,14 @@ __device__ __forceinline__ void row16(const float* p, float (&a)[16]) {
   }
 }
 
-// ---- decays of a chunk.  Lane i of each row of sixteen brings g_i (0 behind the sequence) and takes the running sum c_i as a pair of
-// floats: c_i - c_j is then exact to a rounding of the DIFFERENCE, also behind a step that resets the state (g = -inf counts as
-// -200, whose exponential is 0 in fp32: differences across it vanish, differences behind it do not feel it).
+// ---- decays of a chunk, in powers of two.  Lane i of each row of sixteen brings g_i (0 behind the sequence) and takes the running sum
+// c_i log2(e) as a pair of floats: c_i - c_j is then exact to a rounding of the DIFFERENCE, also behind a step that resets the state
+// (g = -inf counts as -200, whose exponential is 0 in fp32: differences across it vanish, differences behind it do not feel it).
+// v_exp_f32 is good to an ulp; the argument's rounding adds |c_i - c_j| 2^-24, less than the decay's own weight in any sum.
 struct Decay { float hi, lo, enter, leave, whole; };
 __device__ __forceinline__ Decay chunk_decay(float g) {
   if (g < -200.f) g = -200.f;                             // (a nan stays)
-  double c = (double)g;
+  double c = (double)g * 1.4426950408889634;
   c += gd_shr16<1>(c);
   c += gd_shr16<2>(c);
   c += gd_shr16<4>(c);
@@ -164,8 +149,8 @@ __device__ __forceinline__ Decay chunk_decay(float g) {
   d.hi = (float)c;
   d.lo = (float)(c - (double)d.hi);
   const float lh = gd_bcast16<15>(d.hi), ll = gd_bcast16<15>(d.lo);
-  d.enter = expf(d.hi + d.lo);
-  d.leave = expf((lh - d.hi) + (ll - d.lo));
+  d.enter = gd_exp2(d.hi + d.lo);
+  d.leave = gd_exp2((lh - d.hi) + (ll - d.lo));
   d.whole = gd_bcast16<15>(d.enter);
   return d;
 }
@@ -196,6 +181,29 @@ __device__ __forceinline__ Seq seq_of(const Shape& s, int64_t p) {
   q.len = q.live ? len : 0;
   return q;
 }
+// four values of a row in registers as loaded: packed in the storage type until they are used
+template <class IO> struct Quad { int2 x; };
+template <> struct Quad<float> { gd_f4 x; };
+__device__ __forceinline__ gd_f4 unpack(const Quad<float>& q) { return q.x; }
+template <class IO> __device__ __forceinline__ gd_f4 unpack(const Quad<IO>& q) {
+  gd_f4 r;
+  r[0] = to_f32(IO{(uint16_t)((uint32_t)q.x.x & 0xffffu)}); r[1] = to_f32(IO{(uint16_t)((uint32_t)q.x.x >> 16)});
+  r[2] = to_f32(IO{(uint16_t)((uint32_t)q.x.y & 0xffffu)}); r[3] = to_f32(IO{(uint16_t)((uint32_t)q.x.y >> 16)});
+  return r;
+}
+// the first n of four values from p on (the others 0); vec, and always FULL: p is aligned to four values and n is 4 or more, or <= 0
+template <bool FULL> __device__ __forceinline__ void read4(Quad<float>& q, const float* p, int n, bool vec) {
+  if (FULL || vec) { if (n > 0) q.x = lds4(p); else q.x = zero4(); }
+  else q.x = load4(p, n, false);
+}
+template <bool FULL, class IO> __device__ __forceinline__ void read4(Quad<IO>& q, const IO* p, int n, bool vec) {
+  q.x.x = q.x.y = 0;
+  if (FULL || vec) { if (n > 0) q.x = *reinterpret_cast<const int2*>(p); return; }
+  if (n > 0) q.x.x = p[0].u;
+  if (n > 1) q.x.x |= (int)((uint32_t)p[1].u << 16);
+  if (n > 2) q.x.y = p[2].u;
+  if (n > 3) q.x.y |= (int)((uint32_t)p[3].u << 16);
+}
 template <class T> __device__ __forceinline__ const T* at(const View& v, const Seq& q, int h) {
   return reinterpret_cast<const T*>(v.p) + (int64_t)q.b * v.sb + (int64_t)q.n * v.sn + (int64_t)h * v.sh;
 }
@@ -215,9 +223,32 @@ template <int D> struct Team {             // a team of wavefronts owns a sequen
   static constexpr int TEAMS = NW >= 4 ? 1 : 4 / NW;
   static constexpr int TL = 64 * NW;
   static constexpr int THREADS = TL * TEAMS;
+  static constexpr int WAVES = D == 16 ? 4 : D == 32 ? 3 : 2;      // wavefronts a SIMD that the register allocation makes room for
   static constexpr int LD = D + 4;         // LDS row stride: rows of sixteen lanes x 16 bytes cover the banks once
-  static constexpr int EPL = TL >= 256 ? 1 : 256 / TL;      // elements of a 16 x 16 tile a lane
+  static constexpr int SB = D == 128 ? 4 : NW;              // chunks the forward kernel prepares side by side
 };
+// A state [K, V] into / out of the accumulator layout: column n, rows 16 t + 4 cg + r.  Elements outside are read from the state's first
+// value and dropped: a branch around each load would carry the whole register array through it.
+template <int NT, bool FULL> __device__ __forceinline__ void load_state(gd_f4 (&S)[NT], const float* from, int K, int V, int n, int cg) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * t + 4 * cg + r;
+      const bool in = FULL || (row < K && n < V);
+      const float x = from[in ? row * V + n : 0];
+      S[t][r] = in ? x : 0.f;
+    }
+}
+template <int NT, bool FULL> __device__ __forceinline__ void store_state(const gd_f4 (&S)[NT], float* to, int K, int V, int n, int cg) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * t + 4 * cg + r;
+      if (FULL || (row < K && n < V)) to[row * V + n] = S[t][r];
+    }
+}
 template <int D> __device__ __forceinline__ void team_sync() {
   if constexpr (Team<D>::NW == 1) gd_wave_sync(); else gd_block_sync();
 }

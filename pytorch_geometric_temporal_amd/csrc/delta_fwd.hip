@@ -18,21 +18,26 @@ struct FwdArgs {
   int vec;                       // q, k, v rows can be read four values at a time
 };
 
-// One team per sequence and segment of chunks.  PASS 0: outputs.  PASS 1: only the state behind the segment, from a zero start
-// (the first segment: from the sequence's); PASS 2: the segment's transition matrix, i.e. the same recurrence with v = 0 from the unit
-// matrix.  Passes 1 and 2 are what a long sequence with few heads is split with; one launch runs both (blockIdx.z).
-template <class IO, int D, bool TRANS>
-__global__ __launch_bounds__(Team<D>::THREADS) void delta_fwd_kernel(FwdArgs a) {
+// One team per sequence and segment of chunks; a wavefront owns sixteen columns of the state.  Blocks of SB chunks: the tiles that do
+// not depend on the state (P, the inverse, the decays) are prepared first, one chunk a wavefront side by side, then every wavefront walks
+// the block's chunks alone, without a barrier.  A chunk's walk is 3 K / 4 + 8 v_mfma_f32_16x16x4_f32 of 32 cycles, the fp32 matrix
+// pipe's rate: what bounds it at K = 64 and beyond; narrow heads are bound by memory and by the preparation's vector instructions.
+// TRANS: what a long sequence with few heads is split with: blockIdx.z 0: only the state behind the segment, from a zero start (the
+// first segment: from the sequence's); 1: the segment's transition matrix, i.e. the same recurrence with v = 0 from the unit matrix.
+// FULL: K = V = D and rows can be read four values at a time.
+template <class IO, int D, bool TRANS, bool FULL>
+__global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_kernel(FwdArgs a) {
   using TM = Team<D>;
-  constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, EPL = TM::EPL;
+  constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, SB = TM::SB, TB = 16 * SB, NT = D / 16;
   struct Lds {
-    float k[16 * LD], q[16 * LD], v[16 * LD];
-    float part[NW][2][TILE];
-    float am[TILE], pm[TILE];
-    float hi[16], lo[16], enter[16], leave[16], beta[16], whole[4];
+    float k[TB * LD], q[TRANS ? 4 : TB * LD];
+    float inv[SB][256], p[TRANS ? 1 : SB][256];           // A operands, four values a lane
+    float am[NW][TILE];
+    float hi[NW][16], lo[NW][16], enter[SB][16], leave[SB][16], beta[SB][16], whole[SB];
   };
   __shared__ __attribute__((aligned(16))) char smem[sizeof(Lds) * TM::TEAMS];
   const Shape& s = a.s;
+  const int K = FULL ? D : s.K, V = FULL ? D : s.V;
   const int tid = (int)threadIdx.x, team = tid / TL, tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane = tid & 63, col = lane & 15, cg = lane >> 4;
   Lds& L = reinterpret_cast<Lds*>(smem)[team];
   const int64_t first = s.p0 + (int64_t)blockIdx.x * TM::TEAMS;
@@ -42,143 +47,167 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_fwd_kernel(FwdArgs a) 
   if (TRANS && unit && seg == 0) return;
   const int c0 = seg * s.cps, c1 = c0 + s.cps < s.chunks ? c0 + s.cps : s.chunks;
   const int reach = chunks_of_block<TM::TEAMS>(s, first), ce = reach < c1 ? reach : c1;
-  const int kh = sq.h / s.rep, cols = unit ? s.K : s.V;
-  const IO* kp = at<IO>(a.k, sq, kh);
-  const IO* qp = at<IO>(a.q, sq, kh);
-  const IO* vp = at<IO>(a.v, sq, sq.h);
+  const int kh = sq.h / s.rep, cols = unit ? K : V;
   const float* gp = at<float>(a.g, sq, sq.h);
   const float* bp = at<float>(a.beta, sq, sq.h);
-  const bool vec = a.vec != 0;
   const int n = 16 * w + col;                             // this lane's column of the state
-  const bool mine = 16 * w < cols;                        // a wavefront behind the width only helps with the tiles
+  const bool mine = FULL || 16 * w < cols;                // a wavefront behind the width only helps with the tiles
+  const bool vin = FULL || n < V;
 
-  gd_f4 S[QD / 4];
+  gd_f4 S[NT];
+  bool zero = false;                                      // the state is known to be zero
 #pragma unroll
-  for (int t = 0; t < QD / 4; ++t)
+  for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * t + 4 * cg + r;
-      float x = 0.f;
-      if (unit) {
-        x = row == n ? 1.f : 0.f;
-      } else if (sq.live && row < s.K && n < s.V) {
-        if (seg == 0) { if (a.start) x = a.start[(sq.p * s.K + row) * s.V + n]; }
-        else if (!TRANS) x = a.seg_start[((sq.p * (s.segs - 1) + seg - 1) * s.K + row) * s.V + n];
-      }
-      S[t][r] = x;
-    }
+    for (int r = 0; r < 4; ++r) S[t][r] = TRANS && unit && 16 * t + 4 * cg + r == n ? 1.f : 0.f;
+  if (!unit) {
+    const float* from = seg == 0 ? a.start : TRANS ? nullptr : a.seg_start;
+    zero = from == nullptr;
+    if (!zero && sq.live) load_state<NT, FULL>(S, from + (seg == 0 ? sq.p : sq.p * (s.segs - 1) + seg - 1) * K * V, K, V, n, cg);
+  }
 
+  // what the next block brings, in registers: SB quads of k and q a lane, the wavefront's own column of v, the decays of one chunk
   const int tok = tl / QD, qd = 4 * (tl % QD);
-  gd_f4 nk = zero4(), nq = zero4(), nv = zero4();
+  const IO* kp = at<IO>(a.k, sq, kh) + tok * a.k.st + qd;
+  const IO* qp = at<IO>(a.q, sq, kh) + tok * a.q.st + qd;
+  const IO* vp = at<IO>(a.v, sq, sq.h) + 4 * cg * a.v.st + n;
+  Quad<IO> nk[SB], nq[TRANS ? 1 : SB];
+  IO nv[SB][4];
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
-    const int t = 16 * c + tok;
-    const bool in = t < sq.len;
-    nk = load4(kp + (int64_t)t * a.k.st + qd, in ? s.K - qd : 0, vec);
-    if (!TRANS) nq = load4(qp + (int64_t)t * a.q.st + qd, in ? s.K - qd : 0, vec);
-    if (!unit) nv = load4(vp + (int64_t)t * a.v.st + qd, in ? s.V - qd : 0, vec);
-    if (w == 0) {
-      const int tg = 16 * c + col;
-      ng = tg < sq.len ? gp[(int64_t)tg * a.g.st] : 0.f;
-      nb = tg < sq.len ? bp[(int64_t)tg * a.beta.st] : 0.f;
-    }
-  };
-  if (c0 < ce) fetch(c0);
-  for (int c = c0; c < ce; ++c) {
-    put4(&L.k[tok * LD + qd], nk);
-    if (!TRANS) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) nq[r] *= s.scale;
-      put4(&L.q[tok * LD + qd], nq);
+    for (int i = 0; i < SB; ++i) {
+      const int t = 16 * (c + i) + tok;
+      read4<FULL>(nk[i], kp + (int64_t)(16 * (c + i)) * a.k.st, t < sq.len ? K - qd : 0, a.vec != 0);
+      if (!TRANS) read4<FULL>(nq[i], qp + (int64_t)(16 * (c + i)) * a.q.st, t < sq.len ? K - qd : 0, a.vec != 0);
     }
-    put4(&L.v[tok * LD + qd], nv);
-    if (w == 0) {
-      const Decay d = chunk_decay(ng);
-      if (lane < 16) {
-        L.hi[lane] = d.hi; L.lo[lane] = d.lo; L.enter[lane] = d.enter; L.leave[lane] = d.leave; L.beta[lane] = nb;
-        if (lane == 0) L.whole[0] = d.whole;
-      }
-    }
-    if (c + 1 < ce) fetch(c + 1);
-    if (!TRANS && a.states && c > 0 && sq.live) {
-      float* to = a.states + (sq.p * (s.chunks - 1) + c - 1) * s.K * s.V;
+    const int tg = 16 * (c + (SB < NW ? w % SB : w)) + col;
+    ng = nb = 0.f;
+    if (tg < sq.len) { ng = gp[tg * a.g.st]; nb = bp[tg * a.beta.st]; }
+    if (!unit) {
 #pragma unroll
-      for (int t = 0; t < QD / 4; ++t)
+      for (int i = 0; i < SB; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = 16 * t + 4 * cg + r;
-          if (row < s.K && n < s.V) to[(int64_t)row * s.V + n] = S[t][r];
+          const int t = 16 * (c + i) + 4 * cg + r;
+          nv[i][r] = t < sq.len && vin ? vp[(int64_t)(16 * (c + i) + r) * a.v.st] : from_f32<IO>(0.f);
         }
     }
-    team_sync<D>();
-    {   // this wavefront's sixteen key columns of K K^T and Q K^T
-      const gd_f4 kk = lds4(&L.k[col * LD + 16 * w + 4 * cg]);
-      gd_f4 x = mma16(kk, kk, zero4()), y = zero4();
-      if (!TRANS) y = mma16(lds4(&L.q[col * LD + 16 * w + 4 * cg]), kk, zero4());
+  };
+  const int64_t row_v = (int64_t)s.N * s.H * V;           // one step on in o and e
+  const int64_t out0 = ((int64_t)sq.b * s.T * s.N + sq.n) * s.H * V + (int64_t)sq.h * V + 4 * cg * row_v + n;
+  if (c0 < ce) fetch(c0);
+  for (int c = c0; c < ce; c += SB) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        L.part[w][0][(4 * cg + r) * TS + col] = x[r];
-        if (!TRANS) L.part[w][1][(4 * cg + r) * TS + col] = y[r];
+    for (int i = 0; i < SB; ++i) {
+      put4(&L.k[(16 * i + tok) * LD + qd], unpack(nk[i]));
+      if (!TRANS) {
+        gd_f4 x = unpack(nq[i]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] *= s.scale;
+        put4(&L.q[(16 * i + tok) * LD + qd], x);
+      }
+    }
+    gd_f4 v[SB];
+#pragma unroll
+    for (int i = 0; i < SB; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[i][r] = unit ? 0.f : to_f32(nv[i][r]);
+    const float g = ng, b = nb;
+    team_sync<D>();
+    if (c + SB < ce) fetch(c + SB);
+    {   // the tiles of chunk c + i; wavefronts SB .. 2 SB - 1, where there are any, take P off the others
+      const int i = SB < NW ? w % SB : w;
+      const bool do_inv = w < SB, do_p = !TRANS && (SB < NW ? w >= SB : true);
+      const Decay d = chunk_decay(g);
+      if (lane < 16) {
+        L.hi[w][lane] = d.hi; L.lo[w][lane] = d.lo;
+        if (do_inv) { L.enter[i][lane] = d.enter; L.leave[i][lane] = d.leave; L.beta[i][lane] = b; if (lane == 0) L.whole[i] = d.whole; }
+      }
+      gd_f4 kk = zero4(), kq = zero4();                   // row j = 4 cg + r, column i = col: the A operand's layout of the transposed tile
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const gd_f4 x = lds4(&L.k[(16 * i + col) * LD + 16 * t + 4 * cg]);
+        if (do_inv) kk = mma16(x, x, kk);
+        if (do_p) kq = mma16(x, lds4(&L.q[(16 * i + col) * LD + 16 * t + 4 * cg]), kq);
+      }
+      gd_wave_sync();
+      const gd_f4 hj = lds4(&L.hi[w][4 * cg]), lj = lds4(&L.lo[w][4 * cg]);
+      gd_f4 dec;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) dec[r] = 4 * cg + r <= col ? gd_exp2((d.hi - hj[r]) + (d.lo - lj[r])) : 0.f;
+      if (do_p) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kq[r] *= dec[r];
+        put4(&L.p[i][4 * lane], kq);
+      }
+      if (do_inv) {
+        const gd_f4 bj = lds4(&L.beta[i][4 * cg]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kk[r] = 4 * cg + r < col ? dec[r] * kk[r] * bj[r] : 0.f;
+        put4(&L.am[w][col * TS + 4 * cg], kk);
+        gd_wave_sync();
+        float arow[16];
+        row16(&L.am[w][col * TS], arow);
+        gd_f4 inv = unit_row(lane);
+        solve_down<0>(arow, inv);
+        put4(&L.inv[i][4 * lane], inv);
       }
     }
     team_sync<D>();
-    if (tl < 256) {
+#pragma unroll 1                                          // (unrolled, every chunk's LDS reads move to the block's start, and spill)
+    for (int i = 0; i < SB && c + i < ce; ++i) {
+      if (!TRANS && a.states && c + i > 0 && sq.live) {
+        store_state<NT, FULL>(S, a.states + (sq.p * (s.chunks - 1) + c + i - 1) * K * V, K, V, n, cg);
+      }
+      if (!mine) continue;
+      gd_f4 ks = zero4(), o = zero4();
+      const gd_f4 enter = lds4(&L.enter[i][4 * cg]);
+      gd_f4 y = v[0];
 #pragma unroll
-      for (int m = 0; m < EPL; ++m) {
-        const int el = tl + m * TL, i = el >> 4, j = el & 15;
-        float kk = 0.f, qk = 0.f;
+      for (int j = 0; j + 1 < SB; ++j) v[j] = v[j + 1];
+      if (!zero) {
 #pragma unroll
-        for (int u = 0; u < NW; ++u) {
-          kk += L.part[u][0][i * TS + j];
-          if (!TRANS) qk += L.part[u][1][i * TS + j];
+        for (int t = 0; t < NT; ++t) {
+          if (t % 4 == 0) PGT_SCHED_FENCE();
+          ks = mma16(lds4(&L.k[(16 * i + col) * LD + 16 * t + 4 * cg]), S[t], ks);
+          if (!TRANS) o = mma16(lds4(&L.q[(16 * i + col) * LD + 16 * t + 4 * cg]), S[t], o);
         }
-        const float d = j <= i ? expf((L.hi[i] - L.hi[j]) + (L.lo[i] - L.lo[j])) : 0.f;
-        L.am[i * TS + j] = j < i ? d * kk * L.beta[j] : 0.f;
-        if (!TRANS) L.pm[i * TS + j] = j <= i ? d * qk : 0.f;
-      }
-    }
-    team_sync<D>();
-    if (mine) {
-      float arow[16];
-      row16(&L.am[col * TS], arow);
-      gd_f4 inv = unit_row(lane);
-      solve_down<0>(arow, inv);
-      gd_f4 ks = zero4(), qs = zero4();
 #pragma unroll
-      for (int t = 0; t < QD / 4; ++t) {
-        ks = mma16(lds4(&L.k[col * LD + 16 * t + 4 * cg]), S[t], ks);
-        if (!TRANS) qs = mma16(lds4(&L.q[col * LD + 16 * t + 4 * cg]), S[t], qs);
+        for (int r = 0; r < 4; ++r) {
+          y[r] -= enter[r] * ks[r];
+          o[r] *= enter[r];
+        }
       }
-      const gd_f4 enter = lds4(&L.enter[4 * cg]), leave = lds4(&L.leave[4 * cg]), beta = lds4(&L.beta[4 * cg]);
-      gd_f4 y, u, ul;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) y[r] = (unit ? 0.f : L.v[(4 * cg + r) * LD + n]) - enter[r] * ks[r];
-      const gd_f4 e = mma16(inv, y, zero4());
+      const gd_f4 e = mma16(lds4(&L.inv[i][4 * lane]), y, zero4());
+      const gd_f4 leave = lds4(&L.leave[i][4 * cg]), beta = lds4(&L.beta[i][4 * cg]);
+      gd_f4 u, ul;
 #pragma unroll
       for (int r = 0; r < 4; ++r) { u[r] = beta[r] * e[r]; ul[r] = leave[r] * u[r]; }
-      if (!TRANS) {
+      const float whole = L.whole[i];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) qs[r] *= enter[r];
-        const gd_f4 o = mma16(lds4(&L.pm[col * TS + 4 * cg]), u, qs);
-        if (sq.live && n < s.V) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int t = 16 * c + 4 * cg + r;
-            if (t < s.T) {
-              const int64_t off = ((((int64_t)sq.b * s.T + t) * s.N + sq.n) * s.H + sq.h) * s.V + n;
-              reinterpret_cast<IO*>(a.o)[off] = from_f32<IO>(o[r]);
-              if (a.e) a.e[off] = e[r];
-            }
-          }
-        }
-      }
-      const float whole = L.whole[0];
-#pragma unroll
-      for (int t = 0; t < QD / 4; ++t) {
+      for (int t = 0; t < NT; ++t) {
+        if (t % 4 == 0) PGT_SCHED_FENCE();
         gd_f4 kt;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) { kt[r] = L.k[(4 * cg + r) * LD + 16 * t + col]; S[t][r] *= whole; }
+        for (int r = 0; r < 4; ++r) { kt[r] = L.k[(16 * i + 4 * cg + r) * LD + 16 * t + col]; S[t][r] *= whole; }
         S[t] = mma16(kt, ul, S[t]);
+      }
+      zero = false;
+      if (!TRANS) {
+        o = mma16(lds4(&L.p[i][4 * lane]), u, o);
+        if (sq.live && vin) {
+          const int64_t at = out0 + (int64_t)(16 * (c + i)) * row_v;
+          const int left = s.T - 16 * (c + i) - 4 * cg;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < left) reinterpret_cast<IO*>(a.o)[at + r * row_v] = from_f32<IO>(o[r]);
+          if (a.e) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r < left) a.e[at + r * row_v] = e[r];
+          }
+        }
       }
     }
     team_sync<D>();
@@ -186,25 +215,17 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_fwd_kernel(FwdArgs a) 
 
   if (sq.live) {
     float* to;
-    int64_t ld = s.V;
-    if (unit) { to = a.seg_trans + (sq.p * (s.segs - 2) + seg - 1) * s.K * s.K; ld = s.K; }
-    else if (TRANS) to = a.seg_start + (sq.p * (s.segs - 1) + seg) * s.K * s.V;
-    else to = seg == s.segs - 1 ? a.last + sq.p * s.K * s.V : nullptr;
-    if (to) {
-#pragma unroll
-      for (int t = 0; t < QD / 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = 16 * t + 4 * cg + r;
-          if (row < s.K && n < cols) to[(int64_t)row * ld + n] = S[t][r];
-        }
-    }
+    int ld = V;
+    if (unit) { to = a.seg_trans + (sq.p * (s.segs - 2) + seg - 1) * K * K; ld = K; }
+    else if (TRANS) to = a.seg_start + (sq.p * (s.segs - 1) + seg) * K * V;
+    else to = seg == s.segs - 1 ? a.last + sq.p * K * V : nullptr;
+    if (to) store_state<NT, FULL>(S, to, K, ld, n, cg);
     if (!TRANS) {                                         // rows behind the sequence: zero
       const int lo = 16 * (ce > c0 ? ce : c0), hi = 16 * c1 < s.T ? 16 * c1 : s.T;
       for (int t = lo + tok; t < hi; t += 16) {
-        const int64_t off = ((((int64_t)sq.b * s.T + t) * s.N + sq.n) * s.H + sq.h) * s.V;
+        const int64_t off = ((((int64_t)sq.b * s.T + t) * s.N + sq.n) * s.H + sq.h) * V;
         for (int r = 0; r < 4; ++r)
-          if (qd + r < s.V) reinterpret_cast<IO*>(a.o)[off + qd + r] = from_f32<IO>(0.f);
+          if (qd + r < V) reinterpret_cast<IO*>(a.o)[off + qd + r] = from_f32<IO>(0.f);
       }
     }
   }
@@ -212,45 +233,58 @@ __global__ __launch_bounds__(Team<D>::THREADS) void delta_fwd_kernel(FwdArgs a) 
 
 // Joins the segments: the state before segment j + 1 is (transition of segment j) (state before segment j) + (what segment j adds), where
 // x [P, segs - 1, K, V] holds the second summand and takes the sum (its entry 0 is complete already).  UP (the adjoint): from the last
-// entry down with the transposed transitions.  A workgroup owns sixteen columns of a sequence's state; a wavefront sixteen rows.
+// entry down with the transposed transitions.  A workgroup owns sixteen columns of a sequence's state, a wavefront sixteen rows; the
+// next transition is on its way while this one is multiplied: what remains of a step is its K / 4 dependent MFMAs and one barrier.
 template <int D, bool UP>
-__global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K, int V) {
-  constexpr int LD = D + 4;
+__global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K, int V, int vec) {
+  constexpr int LD = D + 4, NT = D / 16;
   __shared__ __attribute__((aligned(16))) float st[2][16 * LD];     // [column][row], two buffers
   const int w = (int)threadIdx.x / 64, lane = (int)threadIdx.x & 63, col = lane & 15, cg = lane >> 4;
   const int64_t p = blockIdx.x;
-  const int n = 16 * (int)blockIdx.y + col, row0 = 16 * w + 4 * cg;
+  const int n = 16 * (int)blockIdx.y + col, row0 = 16 * w + 4 * cg, i = 16 * w + col;
   const int entries = segs - 1;
-  auto value = [&](int j, int r) -> float* { return x + ((p * entries + j) * K + row0 + r) * V + n; };
-  gd_f4 s;
+  float* xp = x + p * entries * K * V + (int64_t)row0 * V + n;
+  const float* mp = trans + p * (segs - 2) * K * K + (UP ? (int64_t)(4 * cg) * K + i : (int64_t)i * K + 4 * cg);
+  gd_f4 m[NT], add;
+  auto fetch = [&](int j) {                               // step j: entry `to` takes the transition of segment `tr`
+    const int to = UP ? entries - 1 - j : j, tr = UP ? entries - j : j;
+    const float* q = mp + (int64_t)(tr - 1) * K * K;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) s[r] = row0 + r < K && n < V ? *value(UP ? entries - 1 : 0, r) : 0.f;
-  for (int j = 1; j < entries; ++j) {
-    const int to = UP ? entries - 1 - j : j;              // entry `to` takes the transition of segment `tr`
-    const int tr = UP ? entries - j : j;
-    const float* m = trans + (p * (segs - 2) + tr - 1) * K * K;
-    float* buf = st[j & 1];
-    put4(&buf[col * LD + row0], s);
-    __syncthreads();
+    for (int t = 0; t < NT; ++t) {
+      const int left = i < K ? K - 16 * t - 4 * cg : 0;
+      if (UP) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = row0 + r < K && n < V ? *value(to, r) : 0.f;
-#pragma unroll
-    for (int t = 0; t < D / 16; ++t) {
-      gd_f4 am;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * w + col, k = 16 * t + 4 * cg + r;
-        am[r] = i < K && k < K ? (UP ? m[(int64_t)k * K + i] : m[(int64_t)i * K + k]) : 0.f;
+        for (int r = 0; r < 4; ++r) m[t][r] = r < left ? q[(int64_t)(16 * t + r) * K] : 0.f;
+      } else {
+        m[t] = load4(q + 16 * t, left, vec != 0);
       }
-      s = mma16(am, lds4(&buf[col * LD + 16 * t + 4 * cg]), s);
     }
 #pragma unroll
+    for (int r = 0; r < 4; ++r) add[r] = row0 + r < K && n < V ? xp[((int64_t)to * K + r) * V] : 0.f;
+  };
+  gd_f4 s;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) s[r] = row0 + r < K && n < V ? xp[((int64_t)(UP ? entries - 1 : 0) * K + r) * V] : 0.f;
+  if (entries > 1) fetch(1);
+  for (int j = 1; j < entries; ++j) {
+    float* buf = st[j & 1];
+    put4(&buf[col * LD + row0], s);
+    s = add;
+    gd_f4 now[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) now[t] = m[t];
+    if (j + 1 < entries) fetch(j + 1);
+    gd_block_sync();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) s = mma16(now[t], lds4(&buf[col * LD + 16 * t + 4 * cg]), s);
+    const int to = UP ? entries - 1 - j : j;
+#pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (row0 + r < K && n < V) *value(to, r) = s[r];
+      if (row0 + r < K && n < V) xp[((int64_t)to * K + r) * V] = s[r];
   }
 }
 
-template <class IO, int D, bool TRANS> void go(const FwdArgs& a0, pgt_stream_t stream) {
+template <class IO, int D, bool TRANS, bool FULL> void go(const FwdArgs& a0, pgt_stream_t stream) {
   using TM = Team<D>;
   FwdArgs a = a0;
   const int64_t most = (int64_t)1 << 21;                  // workgroups of a launch: the grid's threads stay below 2^32
@@ -258,18 +292,19 @@ template <class IO, int D, bool TRANS> void go(const FwdArgs& a0, pgt_stream_t s
     a.s.p0 = p0;
     const int64_t wgs = pgt_cdiv(a.s.P - p0, TM::TEAMS);
     const dim3 grid((unsigned)(wgs < most ? wgs : most), (unsigned)(TRANS ? a.s.segs - 1 : a.s.segs), TRANS && a.s.segs > 2 ? 2 : 1);
-    PGT_LAUNCH((delta_fwd_kernel<IO, D, TRANS>), grid, dim3(TM::THREADS), stream, a);
+    PGT_LAUNCH((delta_fwd_kernel<IO, D, TRANS, FULL>), grid, dim3(TM::THREADS), stream, a);
   }
 }
 template <class IO, int D> void all(const FwdArgs& a, pgt_stream_t stream) {
+  const bool full = a.vec && a.s.K == D && a.s.V == D;
   if (a.s.segs > 1) {
-    go<IO, D, true>(a, stream);
+    if (full) go<IO, D, true, true>(a, stream); else go<IO, D, true, false>(a, stream);
     if (a.s.segs > 2) {
       const dim3 grid((unsigned)a.s.P, (unsigned)((a.s.V + 15) / 16));
-      PGT_LAUNCH((delta_join_kernel<D, false>), grid, dim3(64 * (D / 16)), stream, (const float*)a.seg_trans, a.seg_start, a.s.segs, a.s.K, a.s.V);
+      PGT_LAUNCH((delta_join_kernel<D, false>), grid, dim3(64 * (D / 16)), stream, (const float*)a.seg_trans, a.seg_start, a.s.segs, a.s.K, a.s.V, (int)(a.s.K % 4 == 0 && pgt_aligned(a.seg_trans, 16)));
     }
   }
-  go<IO, D, false>(a, stream);
+  if (full) go<IO, D, false, true>(a, stream); else go<IO, D, false, false>(a, stream);
 }
 template <class IO> void by_width(const FwdArgs& a, pgt_stream_t stream) {
   const int d = a.s.K > a.s.V ? a.s.K : a.s.V;
@@ -284,10 +319,10 @@ template <class IO> void by_width(const FwdArgs& a, pgt_stream_t stream) {
 int pgt_delta_join_up(const float* trans, float* x, int64_t P, int segs, int K, int V, pgt_stream_t stream) {
   const dim3 grid((unsigned)P, (unsigned)((V + 15) / 16));
   const int d = K > V ? K : V;
-  if (d <= 16) PGT_LAUNCH((delta_join_kernel<16, true>), grid, dim3(64), stream, trans, x, segs, K, V);
-  else if (d <= 32) PGT_LAUNCH((delta_join_kernel<32, true>), grid, dim3(128), stream, trans, x, segs, K, V);
-  else if (d <= 64) PGT_LAUNCH((delta_join_kernel<64, true>), grid, dim3(256), stream, trans, x, segs, K, V);
-  else PGT_LAUNCH((delta_join_kernel<128, true>), grid, dim3(512), stream, trans, x, segs, K, V);
+  if (d <= 16) PGT_LAUNCH((delta_join_kernel<16, true>), grid, dim3(64), stream, trans, x, segs, K, V, 0);
+  else if (d <= 32) PGT_LAUNCH((delta_join_kernel<32, true>), grid, dim3(128), stream, trans, x, segs, K, V, 0);
+  else if (d <= 64) PGT_LAUNCH((delta_join_kernel<64, true>), grid, dim3(256), stream, trans, x, segs, K, V, 0);
+  else PGT_LAUNCH((delta_join_kernel<128, true>), grid, dim3(512), stream, trans, x, segs, K, V, 0);
   return pgt_check_launch("pgt_gated_delta_bwd");
 }
 
@@ -313,7 +348,7 @@ int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s) {
   const int64_t wgs = pgt_cdiv(s->P, teams_per_wg);
   int segs = 1;
   if (wgs > 0 && wgs < 128 && s->chunks >= 16) {
-    const int64_t most = 512 / wgs, by_length = s->chunks / 4;
+    const int64_t most = (width > 64 ? 256 : 512) / wgs, by_length = s->chunks / 4;
     segs = (int)(most < by_length ? most : by_length);
     if (segs > 64) segs = 64;
     if (segs < 3) segs = 1;

@@ -32,6 +32,7 @@ template <int N> static inline double gd_shr16(double x) {          // lane i ta
   return (__lane_id() & 15) >= N ? y : 0.0;
 }
 static inline float gd_xsum(float x, int lanes) { for (int m = 1; m < lanes; m <<= 1) x += __shfl_xor(x, m); return x; }
+static inline float gd_exp2(float x) { return exp2f(x); }
 static inline float gd_rcp(float x) { return 1.f / x; }
 static inline float gd_exp(float x) { return expf(x); }
 static inline void gd_wave_sync() { pgt_emu::wave_barrier(); }
