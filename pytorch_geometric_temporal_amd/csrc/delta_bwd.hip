@@ -12,6 +12,8 @@
 // from the forward pass, so the adjoint solves one triangular tile a chunk and runs no forward recurrence.
 #include "delta_common.h"
 
+#include <type_traits>
+
 using namespace gd;
 
 namespace {
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
   __shared__ __attribute__((aligned(16))) char smem[sizeof(Lds) * TM::TEAMS];
   const Shape& s = a.s;
   const int K = FULL ? D : s.K, V = FULL ? D : s.V;
-  const int tid = (int)threadIdx.x, team = tid / TL, tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane = tid & 63, col = lane & 15, cg = lane >> 4;
+  const int tid = (int)threadIdx.x, team = PGT_UNIFORM(tid / TL), tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane = tid & 63, col = lane & 15, cg = lane >> 4;
   Lds& L = reinterpret_cast<Lds*>(smem)[team];
   const int64_t first = s.p0 + (int64_t)blockIdx.x * TM::TEAMS;
   const Seq sq = seq_of(s, first + team);
@@ -81,24 +83,26 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
     if (from && sq.live) load_state<NT, FULL>(S, from + (seg == s.segs - 1 ? sq.p : sq.p * (s.segs - 1) + seg) * K * V, K, V, n, cg);
   }
   const int tok = tl / QD, qd = 4 * (tl % QD);
-  const IO* kp = at<IO>(a.k, sq, kh) + tok * a.k.st + qd;
-  const IO* qp = at<IO>(a.q, sq, kh) + tok * a.q.st + qd;
+  const int nqk = FULL ? 4 : K - qd, nvv = FULL ? 4 : V - qd;      // values of this lane's quads that exist
+  const IO* kp = at<IO>(a.k, sq, kh) + (nqk > 0 ? qd : 0);
+  const IO* qp = at<IO>(a.q, sq, kh) + (nqk > 0 ? qd : 0);
   const int64_t row_v = row_h * V;
-  const IO* op = reinterpret_cast<const IO*>(a.d_o) + seq_h * V + tok * row_v + qd;
-  const float* ep = a.e + seq_h * V + tok * row_v + qd;
-  Quad<IO> nk, nq, no;
-  Quad<float> ne;
+  const IO* op = reinterpret_cast<const IO*>(a.d_o) + seq_h * V + (nvv > 0 ? qd : 0);
+  const float* ep = a.e + seq_h * V + (nvv > 0 ? qd : 0);
+  const int last = s.T - 1;
+  Quad<IO> nk = {}, nq = {}, no = {};
+  Quad<float> ne = {};
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
-    const int64_t t0 = 16 * c;
-    const bool in = t0 + tok < sq.len;
-    read4<FULL>(nk, kp + t0 * a.k.st, in ? K - qd : 0, a.vec != 0);
-    read4<FULL>(nq, qp + t0 * a.q.st, in ? K - qd : 0, a.vec != 0);
-    read4<FULL>(no, op + t0 * row_v, in ? V - qd : 0, a.vec_do != 0);
-    if (!STATE) read4<FULL>(ne, ep + t0 * row_v, in ? V - qd : 0, a.vec_e != 0);
-    const int tg = 16 * c + col;
-    ng = nb = 0.f;
-    if (tg < sq.len) { ng = gp[tg * a.g.st]; nb = bp[tg * a.beta.st]; }
+    int t = 16 * c + tok, tg = 16 * c + col;
+    t = t < last ? t : last;
+    tg = tg < last ? tg : last;
+    read4<FULL>(nk, kp + t * a.k.st, nqk, a.vec != 0);
+    read4<FULL>(nq, qp + t * a.q.st, nqk, a.vec != 0);
+    read4<FULL>(no, op + t * row_v, nvv, a.vec_do != 0);
+    if (!STATE) read4<FULL>(ne, ep + t * row_v, nvv, a.vec_e != 0);
+    ng = gp[tg * a.g.st];
+    nb = bp[tg * a.beta.st];
   };
   // dg and dbeta of chunk c, while the next one's tiles are made, from the row sums in LDS and
   // X_ij = M1_ij q_i.k_j + M2_ij k_i.k_j left of the diagonal (row i = 4 cg + r, column j = col), which wavefront W_DG kept
@@ -139,16 +143,18 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
   };
   if (c0 < ce) fetch(ce - 1);
   for (int c = ce - 1; c >= c0; --c) {
-    put4(&L.k[tok * LD + qd], unpack(nk));
     {
-      gd_f4 x = unpack(nq);
+      const bool in = 16 * c + tok < sq.len;
+      put4(&L.k[tok * LD + qd], unpack<FULL>(nk, in ? nqk : 0));
+      gd_f4 x = unpack<FULL>(nq, in ? nqk : 0);
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] *= s.scale;
       put4(&L.q[tok * LD + qd], x);
+      put4(&L.o[tok * LD + qd], unpack<FULL>(no, in ? nvv : 0));
+      if (!STATE) put4(&L.e[tok * LD + qd], unpack<FULL>(ne, in ? nvv : 0));
     }
-    put4(&L.o[tok * LD + qd], unpack(no));
-    if (!STATE) put4(&L.e[tok * LD + qd], unpack(ne));
-    const float g = ng, b = nb;
+    const bool here = 16 * c + col < sq.len;
+    const float g = here ? ng : 0.f, b = here ? nb : 0.f;
     if (c > c0) fetch(c - 1);
     gd_f4 s0[STATE ? 1 : NT];                             // S0, row = this lane's key column, along the values
     const float* from = c > 0 ? a.states + (sq.p * (s.chunks - 1) + c - 1) * K * V : a.start ? a.start + sq.p * K * V : nullptr;
@@ -234,6 +240,12 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
         put4(&L.inv[4 * lane], inv);
       }
     }
+    arrive(nk);
+    arrive(nq);
+    arrive(no);
+    if (!STATE) arrive(ne);
+    arrive(ng);
+    arrive(nb);
     team_sync<D>();
     // ---- part 2
     const gd_f4 enter = lds4(&L.enter[4 * cg]), leave = lds4(&L.leave[4 * cg]), beta = lds4(&L.beta[4 * cg]);
@@ -285,10 +297,15 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
         }
         if (sq.live && vin) {
           const int64_t at = (seq_h + (int64_t)(16 * c + 4 * cg) * row_h) * V + n;
-          const int left = s.T - 16 * c - 4 * cg;
+          const int left = 16 * c + 16 <= s.T ? 4 : s.T - 16 * c - 4 * cg;
+          if (left >= 4) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r < left) reinterpret_cast<IO*>(a.dv)[at + r * row_v] = from_f32<IO>(dy[r]);
+            for (int r = 0; r < 4; ++r) reinterpret_cast<IO*>(a.dv)[at + r * row_v] = from_f32<IO>(dy[r]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (r < left) reinterpret_cast<IO*>(a.dv)[at + r * row_v] = from_f32<IO>(dy[r]);
+          }
         }
       }
     } else if (!STATE) {                                  // columns behind the values' width: the products below read them
@@ -383,18 +400,23 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
           const int left = s.T - 16 * c - 4 * cg;
           const int64_t row_k = (s.rep > 1 ? row_h : (int64_t)s.N * (s.H / s.rep)) * K;
           const int64_t at = (s.rep > 1 ? seq_h : ((int64_t)sq.b * s.T * s.N + sq.n) * (s.H / s.rep) + kh) * K + (int64_t)(16 * c + 4 * cg) * row_k + n;
+          auto put = [&](auto* dq, auto* dk, int r) {
+            using T = std::remove_pointer_t<decltype(dq)>;
+            dq[at + r * row_k] = from_f32<T>(aq[r] * s.scale);
+            dk[at + r * row_k] = from_f32<T>(ak[r]);
+          };
+          auto rows = [&](auto* dq, auto* dk) {
+            if (16 * c + 16 <= s.T) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if (r < left) {
-              if (s.rep > 1) {
-                reinterpret_cast<float*>(a.dq)[at + r * row_k] = aq[r] * s.scale;
-                reinterpret_cast<float*>(a.dk)[at + r * row_k] = ak[r];
-              } else {
-                reinterpret_cast<IO*>(a.dq)[at + r * row_k] = from_f32<IO>(aq[r] * s.scale);
-                reinterpret_cast<IO*>(a.dk)[at + r * row_k] = from_f32<IO>(ak[r]);
-              }
+              for (int r = 0; r < 4; ++r) put(dq, dk, r);
+            } else {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (r < left) put(dq, dk, r);
             }
-          }
+          };
+          if (s.rep > 1) rows(reinterpret_cast<float*>(a.dq), reinterpret_cast<float*>(a.dk));
+          else rows(reinterpret_cast<IO*>(a.dq), reinterpret_cast<IO*>(a.dk));
         }
       } else if (lane < 16) {
         L.red[w][1][lane] = 0.f;

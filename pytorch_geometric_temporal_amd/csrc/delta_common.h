@@ -172,50 +172,71 @@ __device__ __forceinline__ Seq seq_of(const Shape& s, int64_t p) {
   Seq q;
   q.live = p < s.P;
   q.p = q.live ? p : 0;
-  q.bn = q.p / s.H;
-  q.h = (int)(q.p - q.bn * s.H);
-  q.b = (int)(q.bn / s.N);
-  q.n = (int)(q.bn - (int64_t)q.b * s.N);
+  const uint32_t bn = (uint32_t)q.p / (uint32_t)s.H, b = bn / (uint32_t)s.N;      // (at most 2^31 sequences)
+  q.bn = bn;
+  q.h = (int)((uint32_t)q.p - bn * (uint32_t)s.H);
+  q.b = (int)b;
+  q.n = (int)(bn - b * (uint32_t)s.N);
   int len = s.T;
   if (s.lengths) { len = s.lengths[q.bn]; len = len < 0 ? 0 : len > s.T ? s.T : len; }
   q.len = q.live ? len : 0;
   return q;
 }
-// four values of a row in registers as loaded: packed in the storage type until they are used
+// Four values of a row in registers as loaded: packed in the storage type until they are used.  Every load is issued, from a valid
+// address in any case (row and first value clamped by the caller): a branch around each load costs more than the load.  What is not
+// there is masked when the quad is unpacked: n is how many of the four values exist (FULL, vec: four or none).
 template <class IO> struct Quad { int2 x; };
 template <> struct Quad<float> { gd_f4 x; };
-__device__ __forceinline__ gd_f4 unpack(const Quad<float>& q) { return q.x; }
-template <class IO> __device__ __forceinline__ gd_f4 unpack(const Quad<IO>& q) {
-  gd_f4 r;
-  r[0] = to_f32(IO{(uint16_t)((uint32_t)q.x.x & 0xffffu)}); r[1] = to_f32(IO{(uint16_t)((uint32_t)q.x.x >> 16)});
-  r[2] = to_f32(IO{(uint16_t)((uint32_t)q.x.y & 0xffffu)}); r[3] = to_f32(IO{(uint16_t)((uint32_t)q.x.y >> 16)});
-  return r;
-}
-// the first n of four values from p on (the others 0); vec, and always FULL: p is aligned to four values and n is 4 or more, or <= 0
 template <bool FULL> __device__ __forceinline__ void read4(Quad<float>& q, const float* p, int n, bool vec) {
-  if (FULL || vec) { if (n > 0) q.x = lds4(p); else q.x = zero4(); }
-  else q.x = load4(p, n, false);
+  if (FULL || vec) { q.x = lds4(p); return; }
+  q.x[0] = p[0]; q.x[1] = p[n > 1 ? 1 : 0]; q.x[2] = p[n > 2 ? 2 : 0]; q.x[3] = p[n > 3 ? 3 : 0];
 }
 template <bool FULL, class IO> __device__ __forceinline__ void read4(Quad<IO>& q, const IO* p, int n, bool vec) {
-  q.x.x = q.x.y = 0;
-  if (FULL || vec) { if (n > 0) q.x = *reinterpret_cast<const int2*>(p); return; }
-  if (n > 0) q.x.x = p[0].u;
-  if (n > 1) q.x.x |= (int)((uint32_t)p[1].u << 16);
-  if (n > 2) q.x.y = p[2].u;
-  if (n > 3) q.x.y |= (int)((uint32_t)p[3].u << 16);
+  if (FULL || vec) { q.x = *reinterpret_cast<const int2*>(p); return; }
+  q.x.x = (int)(p[0].u | ((uint32_t)p[n > 1 ? 1 : 0].u << 16));
+  q.x.y = (int)(p[n > 2 ? 2 : 0].u | ((uint32_t)p[n > 3 ? 3 : 0].u << 16));
 }
+template <bool FULL> __device__ __forceinline__ gd_f4 unpack(const Quad<float>& q, int n) {
+  gd_f4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = n > (FULL ? 0 : i) ? q.x[i] : 0.f;
+  return r;
+}
+template <bool FULL, class IO> __device__ __forceinline__ gd_f4 unpack(const Quad<IO>& q, int n) {
+  const uint32_t lo = n > 0 ? (uint32_t)q.x.x : 0u, hi = n > (FULL ? 0 : 2) ? (uint32_t)q.x.y : 0u;
+  gd_f4 r;
+  r[0] = to_f32(IO{(uint16_t)(lo & 0xffffu)}); r[1] = to_f32(IO{(uint16_t)(lo >> 16)});
+  r[2] = to_f32(IO{(uint16_t)(hi & 0xffffu)}); r[3] = to_f32(IO{(uint16_t)(hi >> 16)});
+  if (!FULL) {
+    if (n < 2) r[1] = 0.f;
+    if (n < 4) r[3] = 0.f;
+  }
+  return r;
+}
+// Waits for a load here.  A load that is used behind stores whose number the compiler cannot know would wait for the stores as well.
+#ifdef PGT_EMU
+template <class T> inline void arrive(T&) {}
+#else
+__device__ __forceinline__ void arrive(float& x) { asm volatile("" : "+v"(x)); }
+__device__ __forceinline__ void arrive(bf16& x) { uint32_t t = x.u; asm volatile("" : "+v"(t)); x.u = (uint16_t)t; }
+__device__ __forceinline__ void arrive(f16& x) { uint32_t t = x.u; asm volatile("" : "+v"(t)); x.u = (uint16_t)t; }
+__device__ __forceinline__ void arrive(Quad<float>& q) { asm volatile("" : "+v"(q.x)); }
+template <class IO> __device__ __forceinline__ void arrive(Quad<IO>& q) { asm volatile("" : "+v"(q.x.x), "+v"(q.x.y)); }
+#endif
 template <class T> __device__ __forceinline__ const T* at(const View& v, const Seq& q, int h) {
   return reinterpret_cast<const T*>(v.p) + (int64_t)q.b * v.sb + (int64_t)q.n * v.sn + (int64_t)h * v.sh;
 }
 // chunks that any of the workgroup's sequences reaches (the same in every thread)
 template <int TEAMS> __device__ __forceinline__ int chunks_of_block(const Shape& s, int64_t first) {
+  if (s.lengths == nullptr) return s.chunks;
   int most = 0;
 #pragma unroll
   for (int i = 0; i < TEAMS; ++i) {
-    const int len = seq_of(s, first + i).len;
+    if (first + i >= s.P) break;
+    const int len = s.lengths[(uint32_t)(first + i) / (uint32_t)s.H];
     most = len > most ? len : most;
   }
-  return (most + 15) / 16;
+  return ((most < s.T ? most : s.T) + 15) / 16;
 }
 
 template <int D> struct Team {             // a team of wavefronts owns a sequence: one wavefront to 16 columns of the padded width

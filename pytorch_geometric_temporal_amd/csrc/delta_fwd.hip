@@ -38,7 +38,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
   __shared__ __attribute__((aligned(16))) char smem[sizeof(Lds) * TM::TEAMS];
   const Shape& s = a.s;
   const int K = FULL ? D : s.K, V = FULL ? D : s.V;
-  const int tid = (int)threadIdx.x, team = tid / TL, tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane = tid & 63, col = lane & 15, cg = lane >> 4;
+  const int tid = (int)threadIdx.x, team = PGT_UNIFORM(tid / TL), tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane = tid & 63, col = lane & 15, cg = lane >> 4;
   Lds& L = reinterpret_cast<Lds*>(smem)[team];
   const int64_t first = s.p0 + (int64_t)blockIdx.x * TM::TEAMS;
   const Seq sq = seq_of(s, first + team);
@@ -68,29 +68,34 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
 
   // what the next block brings, in registers: SB quads of k and q a lane, the wavefront's own column of v, the decays of one chunk
   const int tok = tl / QD, qd = 4 * (tl % QD);
-  const IO* kp = at<IO>(a.k, sq, kh) + tok * a.k.st + qd;
-  const IO* qp = at<IO>(a.q, sq, kh) + tok * a.q.st + qd;
-  const IO* vp = at<IO>(a.v, sq, sq.h) + 4 * cg * a.v.st + n;
-  Quad<IO> nk[SB], nq[TRANS ? 1 : SB];
-  IO nv[SB][4];
+  const int nqk = FULL ? 4 : K - qd;                      // values of this lane's quad that exist
+  const IO* kp = at<IO>(a.k, sq, kh) + (nqk > 0 ? qd : 0);
+  const IO* qp = at<IO>(a.q, sq, kh) + (nqk > 0 ? qd : 0);
+  const IO* vp = at<IO>(a.v, sq, sq.h) + (vin ? n : 0);
+  const int last = s.T - 1;
+  Quad<IO> nk[SB] = {}, nq[TRANS ? 1 : SB] = {};
+  IO nv[SB][4] = {};
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
-      const int t = 16 * (c + i) + tok;
-      read4<FULL>(nk[i], kp + (int64_t)(16 * (c + i)) * a.k.st, t < sq.len ? K - qd : 0, a.vec != 0);
-      if (!TRANS) read4<FULL>(nq[i], qp + (int64_t)(16 * (c + i)) * a.q.st, t < sq.len ? K - qd : 0, a.vec != 0);
+      int t = 16 * (c + i) + tok;
+      t = t < last ? t : last;
+      read4<FULL>(nk[i], kp + t * a.k.st, nqk, a.vec != 0);
+      if (!TRANS) read4<FULL>(nq[i], qp + t * a.q.st, nqk, a.vec != 0);
     }
-    const int tg = 16 * (c + (SB < NW ? w % SB : w)) + col;
-    ng = nb = 0.f;
-    if (tg < sq.len) { ng = gp[tg * a.g.st]; nb = bp[tg * a.beta.st]; }
+    int tg = 16 * (c + (SB < NW ? w % SB : w)) + col;
+    tg = tg < last ? tg : last;
+    ng = gp[tg * a.g.st];
+    nb = bp[tg * a.beta.st];
     if (!unit) {
 #pragma unroll
       for (int i = 0; i < SB; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int t = 16 * (c + i) + 4 * cg + r;
-          nv[i][r] = t < sq.len && vin ? vp[(int64_t)(16 * (c + i) + r) * a.v.st] : from_f32<IO>(0.f);
+          int t = 16 * (c + i) + 4 * cg + r;
+          t = t < last ? t : last;
+          nv[i][r] = vp[t * a.v.st];
         }
     }
   };
@@ -100,9 +105,10 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
   for (int c = c0; c < ce; c += SB) {
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
-      put4(&L.k[(16 * i + tok) * LD + qd], unpack(nk[i]));
+      const int have = 16 * (c + i) + tok < sq.len ? nqk : 0;
+      put4(&L.k[(16 * i + tok) * LD + qd], unpack<FULL>(nk[i], have));
       if (!TRANS) {
-        gd_f4 x = unpack(nq[i]);
+        gd_f4 x = unpack<FULL>(nq[i], have);
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] *= s.scale;
         put4(&L.q[(16 * i + tok) * LD + qd], x);
@@ -112,13 +118,14 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
 #pragma unroll
     for (int i = 0; i < SB; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[i][r] = unit ? 0.f : to_f32(nv[i][r]);
-    const float g = ng, b = nb;
+      for (int r = 0; r < 4; ++r) v[i][r] = !unit && vin && 16 * (c + i) + 4 * cg + r < sq.len ? to_f32(nv[i][r]) : 0.f;
+    const bool here = 16 * (c + (SB < NW ? w % SB : w)) + col < sq.len;
+    const float g = here ? ng : 0.f, b = here ? nb : 0.f;
     team_sync<D>();
     if (c + SB < ce) fetch(c + SB);
     {   // the tiles of chunk c + i; wavefronts SB .. 2 SB - 1, where there are any, take P off the others
       const int i = SB < NW ? w % SB : w;
-      const bool do_inv = w < SB, do_p = !TRANS && (SB < NW ? w >= SB : true);
+      const bool do_inv = SB < NW ? w < SB : true, do_p = !TRANS && (SB < NW ? w >= SB : true);
       const Decay d = chunk_decay(g);
       if (lane < 16) {
         L.hi[w][lane] = d.hi; L.lo[w][lane] = d.lo;
@@ -154,6 +161,15 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
         put4(&L.inv[i][4 * lane], inv);
       }
     }
+#pragma unroll
+    for (int i = 0; i < SB; ++i) {
+      arrive(nk[i]);
+      if (!TRANS) arrive(nq[i]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) arrive(nv[i][r]);
+    }
+    arrive(ng);
+    arrive(nb);
     team_sync<D>();
 #pragma unroll 1                                          // (unrolled, every chunk's LDS reads move to the block's start, and spill)
     for (int i = 0; i < SB && c + i < ce; ++i) {
@@ -161,8 +177,12 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
         store_state<NT, FULL>(S, a.states + (sq.p * (s.chunks - 1) + c + i - 1) * K * V, K, V, n, cg);
       }
       if (!mine) continue;
+      const gd_f4 enter = lds4(&L.enter[i][4 * cg]), leave = lds4(&L.leave[i][4 * cg]), beta = lds4(&L.beta[i][4 * cg]);
+      const gd_f4 inv = lds4(&L.inv[i][4 * lane]);
+      gd_f4 pm = zero4();
+      if (!TRANS) pm = lds4(&L.p[i][4 * lane]);
+      const float whole = L.whole[i];
       gd_f4 ks = zero4(), o = zero4();
-      const gd_f4 enter = lds4(&L.enter[i][4 * cg]);
       gd_f4 y = v[0];
 #pragma unroll
       for (int j = 0; j + 1 < SB; ++j) v[j] = v[j + 1];
@@ -179,12 +199,10 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
           o[r] *= enter[r];
         }
       }
-      const gd_f4 e = mma16(lds4(&L.inv[i][4 * lane]), y, zero4());
-      const gd_f4 leave = lds4(&L.leave[i][4 * cg]), beta = lds4(&L.beta[i][4 * cg]);
+      const gd_f4 e = mma16(inv, y, zero4());
       gd_f4 u, ul;
 #pragma unroll
       for (int r = 0; r < 4; ++r) { u[r] = beta[r] * e[r]; ul[r] = leave[r] * u[r]; }
-      const float whole = L.whole[i];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (t % 4 == 0) PGT_SCHED_FENCE();
@@ -195,17 +213,26 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
       }
       zero = false;
       if (!TRANS) {
-        o = mma16(lds4(&L.p[i][4 * lane]), u, o);
+        o = mma16(pm, u, o);
         if (sq.live && vin) {
           const int64_t at = out0 + (int64_t)(16 * (c + i)) * row_v;
           const int left = s.T - 16 * (c + i) - 4 * cg;
+          IO* op = reinterpret_cast<IO*>(a.o) + at;
+          float* ep = a.e + at;
+          if (16 * (c + i) + 16 <= s.T) {                 // a whole chunk: no lane asks
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (r < left) reinterpret_cast<IO*>(a.o)[at + r * row_v] = from_f32<IO>(o[r]);
-          if (a.e) {
+            for (int r = 0; r < 4; ++r) op[r * row_v] = from_f32<IO>(o[r]);
+            if (a.e) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) ep[r * row_v] = e[r];
+            }
+          } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (r < left) a.e[at + r * row_v] = e[r];
+              if (r < left) {
+                op[r * row_v] = from_f32<IO>(o[r]);
+                if (a.e) ep[r * row_v] = e[r];
+              }
           }
         }
       }
