@@ -59,13 +59,9 @@ class DeltaDimsStruct(ctypes.Structure):
                 ("key", ctypes.c_int32), ("value", ctypes.c_int32), ("dtype", ctypes.c_int32), ("scale", c_f32), ("lengths", c_ptr)]
 
 
-class SeqViewStruct(ctypes.Structure):
-    """pgt_seq_view: element strides of [batch, step, node, head]."""
-    _fields_ = [("data", c_ptr), ("batch", c_i64), ("step", c_i64), ("node", c_i64), ("head", c_i64)]
-
-
 c_dims = ctypes.POINTER(DeltaDimsStruct)
-c_view = ctypes.POINTER(SeqViewStruct)
+c_view = c_ptr                        # const pgt_seq_view*: the host address of five int64 (data, strides of batch, step, node, head)
+SeqViews5 = c_i64 * 25                # the views of q, k, v, g, beta side by side: one object to build a call
 
 
 class SymGraphStruct(ctypes.Structure):

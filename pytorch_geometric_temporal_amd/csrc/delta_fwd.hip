@@ -1,5 +1,6 @@
 // Gated delta rule, whole sequences, forward (delta_common.h has the formulas).
 #include "delta_common.h"
+#include <stdlib.h>
 
 using namespace gd;
 
@@ -26,7 +27,7 @@ struct FwdArgs {
 // first segment: from the sequence's); 1: the segment's transition matrix, i.e. the same recurrence with v = 0 from the unit matrix.
 // FULL: K = V = D and rows can be read four values at a time.
 template <class IO, int D, bool TRANS, bool FULL>
-__global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void delta_fwd_kernel(FwdArgs a) {
   using TM = Team<D>;
   constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, SB = TM::SB, TB = 16 * SB, NT = D / 16;
   struct Lds {
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_fwd_ke
 // Joins the segments: the state before segment j + 1 is (transition of segment j) (state before segment j) + (what segment j adds), where
 // x [P, segs - 1, K, V] holds the second summand and takes the sum (its entry 0 is complete already).  UP (the adjoint): from the last
 // entry down with the transposed transitions.  A workgroup owns sixteen columns of a sequence's state, a wavefront sixteen rows; the
-// next transition is on its way while this one is multiplied: what remains of a step is its K / 4 dependent MFMAs and one barrier.
+// next two transitions are on their way while one is multiplied: what remains of a step is its K / 4 dependent MFMAs and one barrier.
 template <int D, bool UP>
 __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K, int V, int vec) {
   constexpr int LD = D + 4, NT = D / 16;
@@ -270,45 +271,60 @@ __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* 
   const int64_t p = blockIdx.x;
   const int n = 16 * (int)blockIdx.y + col, row0 = 16 * w + 4 * cg, i = 16 * w + col;
   const int entries = segs - 1;
-  float* xp = x + p * entries * K * V + (int64_t)row0 * V + n;
-  const float* mp = trans + p * (segs - 2) * K * K + (UP ? (int64_t)(4 * cg) * K + i : (int64_t)i * K + 4 * cg);
-  gd_f4 m[NT], add;
-  auto fetch = [&](int j) {                               // step j: entry `to` takes the transition of segment `tr`
+  float* x0 = x + p * entries * K * V;
+  float* xp = x0 + (int64_t)row0 * V + n;
+  const float* mp = trans + p * (segs - 2) * K * K;
+  const int at_m = UP ? 4 * cg * K + i : i * K + 4 * cg;
+  gd_f4 m0[NT], m1[NT], add0, add1;
+  auto fetch = [&](int j, gd_f4 (&m)[NT], gd_f4& add) {                               // step j: entry `to` takes the transition of segment `tr`
     const int to = UP ? entries - 1 - j : j, tr = UP ? entries - j : j;
     const float* q = mp + (int64_t)(tr - 1) * K * K;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+    for (int t = 0; t < NT; ++t) {                        // (elements outside: the matrix's own first value, masked)
       const int left = i < K ? K - 16 * t - 4 * cg : 0;
-      if (UP) {
+      if (!UP && vec) {
+        const gd_f4 x = lds4(q + (left > 0 ? at_m + 16 * t : 0));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) m[t][r] = r < left ? q[(int64_t)(16 * t + r) * K] : 0.f;
+        for (int r = 0; r < 4; ++r) m[t][r] = left > 0 ? x[r] : 0.f;
       } else {
-        m[t] = load4(q + 16 * t, left, vec != 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = q[r < left ? (UP ? at_m + (16 * t + r) * K : at_m + 16 * t + r) : 0];
+          m[t][r] = r < left ? x : 0.f;
+        }
       }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) add[r] = row0 + r < K && n < V ? xp[((int64_t)to * K + r) * V] : 0.f;
+    for (int r = 0; r < 4; ++r) {
+      const bool in = row0 + r < K && n < V;
+      const float x = x0[(int64_t)to * K * V + (in ? (row0 + r) * V + n : 0)];
+      add[r] = in ? x : 0.f;
+    }
   };
   gd_f4 s;
 #pragma unroll
   for (int r = 0; r < 4; ++r) s[r] = row0 + r < K && n < V ? xp[((int64_t)(UP ? entries - 1 : 0) * K + r) * V] : 0.f;
-  if (entries > 1) fetch(1);
-  for (int j = 1; j < entries; ++j) {
+  auto step = [&](int j, gd_f4 (&m)[NT], gd_f4& add) {
     float* buf = st[j & 1];
     put4(&buf[col * LD + row0], s);
-    s = add;
-    gd_f4 now[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) now[t] = m[t];
-    if (j + 1 < entries) fetch(j + 1);
     gd_block_sync();
+    s = add;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) s = mma16(now[t], lds4(&buf[col * LD + 16 * t + 4 * cg]), s);
+    for (int t = 0; t < NT; ++t) s = mma16(m[t], lds4(&buf[col * LD + 16 * t + 4 * cg]), s);
     const int to = UP ? entries - 1 - j : j;
+    fetch(j + 2 < entries ? j + 2 : entries - 1, m, add);  // (always: with a branch here every step would wait for all loads)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (row0 + r < K && n < V) xp[((int64_t)to * K + r) * V] = s[r];
+  };
+  fetch(1, m0, add0);
+  fetch(entries > 2 ? 2 : 1, m1, add1);
+  int j = 1;
+  for (; j + 1 < entries; j += 2) {
+    step(j, m0, add0);
+    step(j + 1, m1, add1);
   }
+  if (j < entries) step(j, m0, add0);
 }
 
 template <class IO, int D, bool TRANS, bool FULL> void go(const FwdArgs& a0, pgt_stream_t stream) {
@@ -374,8 +390,9 @@ int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s) {
   const int64_t teams_per_wg = width <= 16 ? 4 : width <= 32 ? 2 : 1;
   const int64_t wgs = pgt_cdiv(s->P, teams_per_wg);
   int segs = 1;
-  if (wgs > 0 && wgs < 128 && s->chunks >= 16) {
-    const int64_t most = (width > 64 ? 256 : 512) / wgs, by_length = s->chunks / 4;
+  static const int lim = getenv("GD_LIM") ? atoi(getenv("GD_LIM")) : 512, mst = getenv("GD_MOST") ? atoi(getenv("GD_MOST")) : 2048, m128 = getenv("GD_M128") ? atoi(getenv("GD_M128")) : 256;
+  if (wgs > 0 && wgs < lim && s->chunks >= 16) {
+    const int64_t most = (width > 64 ? m128 : mst) / wgs, by_length = s->chunks / 4;
     segs = (int)(most < by_length ? most : by_length);
     if (segs > 64) segs = 64;
     if (segs < 3) segs = 1;

@@ -1,12 +1,13 @@
 """Gated delta rule: whole sequences with gradients, and one step with the state in place.
 (One family of `pytorch_geometric_temporal_amd.ops`; the package re-exports every name and forwards writes to its switches.)
 """
+import contextlib
 import ctypes
 
 import torch
 
 from .. import _lib
-from .._lib import DeltaDimsStruct, SeqViewStruct, check_tensor, ptr, stream_of
+from .._lib import DeltaDimsStruct, SeqViews5, check_tensor, ptr, stream_of
 
 F32 = torch.float32
 
@@ -16,40 +17,53 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MAX_HEAD_WIDTH = 128
 
 
-def _view(t, step):
-    """pgt_seq_view of [B, T, N, H(, C)] (step) or [B, N, H(, C)]."""
-    st = t.stride()
-    v = SeqViewStruct(t.data_ptr(), st[0], st[1], st[2], st[3]) if step else SeqViewStruct(t.data_ptr(), st[0], 0, st[1], st[2])
-    return ctypes.byref(v)
+def _views(q, k, v, g, beta):
+    """pgt_seq_view of [B, T, N, H, C] tensors (g, beta: [B, T, N, H]), or of [B, N, H, C] ones without a step axis: the array that
+    holds them (keep it until the call returns) and the five host addresses."""
+    vals = []
+    for t in (q, k, v, g, beta):
+        vals.append(t.data_ptr())
+        vals += t.stride()[:4] if v.dim() == 5 else (t.stride(0), 0, t.stride(1), t.stride(2))
+    arr = SeqViews5(*vals)
+    at = ctypes.addressof(arr)
+    return arr, (at, at + 40, at + 80, at + 120, at + 160)
 
 
 def _last_axis_contiguous(t):
-    return t if t.size(-1) <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.size(-1) <= 1 else t.contiguous()
+
+
+def on_device(t):
+    """The tensor's device as the current one, where it is not (a launch goes to a stream of the current device)."""
+    return contextlib.nullcontext() if not t.is_cuda or t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def _check(lib, what, q, k, v, g, beta, lead):
     """Types, devices and shapes of an operator's inputs; returns (k_heads, heads, key, value)."""
     if not isinstance(v, torch.Tensor) or v.dtype not in DTYPES:
         raise TypeError(f"{what}: v must be a float32, bfloat16 or float16 tensor, got {getattr(v, 'dtype', type(v))}")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        check_tensor(lib, t, f"{what}: {name}", v.dtype)
-    for t, name in ((g, "g"), (beta, "beta")):
-        check_tensor(lib, t, f"{what}: {name}")
-    if v.dim() != lead + 2 or q.dim() != lead + 2 or q.shape[:lead] != v.shape[:lead]:
+    dtype, device = v.dtype, v.device
+    check_tensor(lib, v, f"{what}: v", dtype)
+    for t, name, want in ((q, "q", dtype), (k, "k", dtype), (g, "g", F32), (beta, "beta", F32)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} must be a tensor")
+        if t.dtype != want:
+            raise TypeError(f"{what}: {name} must be {want}, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{what}: inputs on {t.device} and {device}")
+    qs, vs = q.shape, v.shape
+    if len(vs) != lead + 2 or len(qs) != lead + 2 or qs[:lead] != vs[:lead]:
         axes = "[batch, steps, nodes, heads, width]" if lead == 3 else "[batch, nodes, heads, width]"
-        raise ValueError(f"{what}: q, k, v must be {axes} with the same leading axes, got q {tuple(q.shape)}, v {tuple(v.shape)}")
-    if k.shape != q.shape:
-        raise ValueError(f"{what}: k {tuple(k.shape)} must have q's shape {tuple(q.shape)}")
-    if g.shape != v.shape[:-1] or beta.shape != v.shape[:-1]:
-        raise ValueError(f"{what}: g {tuple(g.shape)} and beta {tuple(beta.shape)} must be {tuple(v.shape[:-1])}")
-    Hk, K, H, V = q.size(-2), q.size(-1), v.size(-2), v.size(-1)
+        raise ValueError(f"{what}: q, k, v must be {axes} with the same leading axes, got q {tuple(qs)}, v {tuple(vs)}")
+    if k.shape != qs:
+        raise ValueError(f"{what}: k {tuple(k.shape)} must have q's shape {tuple(qs)}")
+    if g.shape != vs[:-1] or beta.shape != vs[:-1]:
+        raise ValueError(f"{what}: g {tuple(g.shape)} and beta {tuple(beta.shape)} must be {tuple(vs[:-1])}")
+    Hk, K, H, V = qs[-2], qs[-1], vs[-2], vs[-1]
     if Hk < 1 or H < 1 or H % Hk:
         raise ValueError(f"{what}: {H} value heads do not divide over {Hk} key heads")
     if not (1 <= K <= MAX_HEAD_WIDTH and 1 <= V <= MAX_HEAD_WIDTH):
         raise ValueError(f"{what}: head widths must be 1 .. {MAX_HEAD_WIDTH}, got key {K}, value {V}")
-    for t in (q, k, g, beta):
-        if t.device != v.device:
-            raise ValueError(f"{what}: inputs on {t.device} and {v.device}")
     return Hk, H, K, V
 
 
@@ -61,33 +75,38 @@ def _check_state(lib, what, name, t, shape, device):
         raise ValueError(f"{what}: {name} is on {t.device}, the inputs on {device}")
 
 
+def _forward(q, k, v, g, beta, start, lengths, scale, keep):
+    """pgt_gated_delta_fwd: (o, last, what the adjoint needs if `keep`)."""
+    lib = _lib.get_lib()
+    B, T, N, H, V = v.shape
+    Hk, K = q.shape[3:]
+    dev, P = v.device, B * N * H
+    dims = DeltaDimsStruct(B, T, N, Hk, H, K, V, DTYPES[v.dtype], scale, ptr(lengths))
+    segs = lib._pgt_gated_delta_segments(dims)
+    if segs < 0:
+        raise _lib.PgtError(f"gated_delta_rule: {lib.last_error()}")
+    o = torch.empty(B, T, N, H, V, dtype=v.dtype, device=dev)
+    last = torch.empty(B, N, H, K, V, dtype=F32, device=dev)
+    e = torch.empty(B, T, N, H, V, dtype=F32, device=dev) if keep else None
+    states = torch.empty(P, (T + 15) // 16 - 1, K, V, dtype=F32, device=dev) if keep and T > 16 else None
+    seg_start = torch.empty(P, segs - 1, K, V, dtype=F32, device=dev) if segs > 1 else None
+    seg_trans = torch.empty(P, segs - 2, K, K, dtype=F32, device=dev) if segs > 1 else None
+    arr, views = _views(q, k, v, g, beta)
+    _timed("gated_delta", 7.0 * P * T * K * V if KERNEL_TIMER else 0, lambda: lib.call(
+        "pgt_gated_delta_fwd", dims, *views, ptr(start), ptr(o), ptr(last), ptr(e), ptr(states), ptr(seg_start), ptr(seg_trans),
+        stream_of(lib, v)))
+    return o, last, (e, states, seg_trans)
+
+
 class GatedDeltaFunction(torch.autograd.Function):
     """pgt_gated_delta_fwd / pgt_gated_delta_bwd.  For the adjoint the forward pass keeps the misses e and the state before every
     sixteenth step; with few sequences and many steps also the segments' transitions (pgt_gated_delta_segments)."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, start, lengths, scale):
-        lib = _lib.get_lib()
-        B, T, N, H, V = v.shape
-        Hk, K = q.shape[3:]
-        dev, P = v.device, B * N * H
-        dims = DeltaDimsStruct(B, T, N, Hk, H, K, V, DTYPES[v.dtype], scale, ptr(lengths))
-        segs = lib._pgt_gated_delta_segments(ctypes.byref(dims))
-        if segs < 0:
-            raise _lib.PgtError(f"gated_delta_rule: {lib.last_error()}")
-        need = any(ctx.needs_input_grad)
-        o = torch.empty(B, T, N, H, V, dtype=v.dtype, device=dev)
-        last = torch.empty(B, N, H, K, V, dtype=F32, device=dev)
-        e = torch.empty(B, T, N, H, V, dtype=F32, device=dev) if need else None
-        states = torch.empty(P, max((T + 15) // 16 - 1, 0), K, V, dtype=F32, device=dev) if need else None
-        seg_start = torch.empty(P, segs - 1, K, V, dtype=F32, device=dev) if segs > 1 else None
-        seg_trans = torch.empty(P, segs - 2, K, K, dtype=F32, device=dev) if segs > 1 else None
-        _timed("gated_delta", 7.0 * P * T * K * V if KERNEL_TIMER else 0, lambda: lib.call(
-            "pgt_gated_delta_fwd", ctypes.byref(dims), _view(q, True), _view(k, True), _view(v, True), _view(g, True), _view(beta, True),
-            ptr(start), ptr(o), ptr(last), ptr(e), ptr(states), ptr(seg_start), ptr(seg_trans), stream_of(lib, v)))
-        if need:
-            ctx.save_for_backward(q, k, g, beta, start, lengths, e, states, seg_trans)
-            ctx.dims = (B, T, N, Hk, H, K, V, v.dtype, scale, segs)
+        o, last, kept = _forward(q, k, v, g, beta, start, lengths, scale, True)
+        ctx.save_for_backward(q, k, g, beta, start, lengths, *kept)
+        ctx.like, ctx.scale = (v.size(3), v.size(4)), scale
         ctx.set_materialize_grads(False)
         return o, last
 
@@ -96,8 +115,9 @@ class GatedDeltaFunction(torch.autograd.Function):
     def backward(ctx, d_o, d_last):
         lib = _lib.get_lib()
         q, k, g, beta, start, lengths, e, states, seg_trans = ctx.saved_tensors
-        B, T, N, Hk, H, K, V, dtype, scale, segs = ctx.dims
-        dev, P = q.device, B * N * H
+        B, T, N, Hk, K = q.shape
+        (H, V), scale, dtype, dev = ctx.like, ctx.scale, q.dtype, q.device
+        P, segs = B * N * H, 1 if seg_trans is None else seg_trans.size(1) + 2
         if d_o is None and d_last is None:
             return (None,) * 8
         d_o = torch.zeros(B, T, N, H, V, dtype=dtype, device=dev) if d_o is None else d_o.contiguous()
@@ -111,10 +131,10 @@ class GatedDeltaFunction(torch.autograd.Function):
         head_ws = torch.empty(2, P * T * K, dtype=F32, device=dev) if H > Hk else None
         seg_end = torch.empty(P, segs - 1, K, V, dtype=F32, device=dev) if segs > 1 else None
         dims = DeltaDimsStruct(B, T, N, Hk, H, K, V, DTYPES[dtype], scale, ptr(lengths))
+        arr, (qv, kv, _, gv, bv) = _views(q, k, d_o, g, beta)
         _timed("gated_delta_bwd", 14.0 * P * T * K * V if KERNEL_TIMER else 0, lambda: lib.call(
-            "pgt_gated_delta_bwd", ctypes.byref(dims), _view(q, True), _view(k, True), _view(g, True), _view(beta, True), ptr(start),
-            ptr(e), ptr(states), ptr(seg_trans), ptr(d_o), ptr(d_last), ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(dbeta), ptr(d_start),
-            ptr(head_ws), ptr(seg_end), stream_of(lib, q)))
+            "pgt_gated_delta_bwd", dims, qv, kv, gv, bv, ptr(start), ptr(e), ptr(states), ptr(seg_trans), ptr(d_o), ptr(d_last), ptr(dq),
+            ptr(dk), ptr(dv), ptr(dg), ptr(dbeta), ptr(d_start), ptr(head_ws), ptr(seg_end), stream_of(lib, q)))
         return dq, dk, dv, dg, dbeta, d_start, None, None
 
 
@@ -148,8 +168,12 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, lengths=None, scale=N
             raise ValueError(f"{what}: lengths must be [{B}] or [{B}, {N}], got {tuple(lengths.shape)}")
         lengths = (lengths if lengths.dim() == 2 else lengths[:, None]).clamp(0, T).to(torch.int32).expand(B, N).contiguous()
     scale = float(K) ** -0.5 if scale is None else float(scale)
-    with torch.cuda.device_of(v):
-        return GatedDeltaFunction.apply(*(_last_axis_contiguous(t) for t in (q, k, v)), g, beta, initial_state, lengths, scale)
+    q, k, v = _last_axis_contiguous(q), _last_axis_contiguous(k), _last_axis_contiguous(v)
+    with on_device(v):
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
+                                        or initial_state is not None and initial_state.requires_grad):
+            return GatedDeltaFunction.apply(q, k, v, g, beta, initial_state, lengths, scale)
+        return _forward(q, k, v, g, beta, initial_state, lengths, scale, False)[:2]
 
 
 def gated_delta_step(q, k, v, g, beta, state, scale=None):
@@ -162,13 +186,17 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None):
     _check_state(lib, what, "state", state, (B, N, H, K, V), v.device)
     if not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous (it is updated in place)")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
+                                    or state.requires_grad):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad(), or use gated_delta_rule")
-    q, k, v = (_last_axis_contiguous(t) for t in (q, k, v))
+    q, k, v = _last_axis_contiguous(q), _last_axis_contiguous(k), _last_axis_contiguous(v)
     o = torch.empty(B, N, H, V, dtype=v.dtype, device=v.device)
     dims = DeltaDimsStruct(B, 1, N, Hk, H, K, V, DTYPES[v.dtype], float(K) ** -0.5 if scale is None else float(scale), None)
-    with torch.cuda.device_of(v):
-        _timed("gated_delta_step", 8.0 * state.numel() if KERNEL_TIMER else 0, lambda: lib.call(
-            "pgt_gated_delta_step", ctypes.byref(dims), _view(q, False), _view(k, False), _view(v, False), _view(g, False),
-            _view(beta, False), ptr(state), ptr(o), stream_of(lib, v)))
+    arr, views = _views(q, k, v, g, beta)
+    with on_device(v):
+        if KERNEL_TIMER is None:
+            lib.call("pgt_gated_delta_step", dims, *views, state.data_ptr(), o.data_ptr(), stream_of(lib, v))
+        else:
+            _timed("gated_delta_step", 8.0 * state.numel(), lambda: lib.call(
+                "pgt_gated_delta_step", dims, *views, state.data_ptr(), o.data_ptr(), stream_of(lib, v)))
     return o

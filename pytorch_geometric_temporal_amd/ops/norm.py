@@ -9,28 +9,36 @@ from .._lib import check_tensor, ptr, stream_of
 F32 = torch.float32
 
 from ._core import KERNEL_TIMER, _timed
-from .delta import DTYPES
+from .delta import DTYPES, on_device
 
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2}
 
 
+def _forward(x, B, S, C, groups, weight, bias, eps, act, keep):
+    """pgt_group_norm_act on x [B, .., C] contiguous: y, and the statistics the adjoint needs if `keep`."""
+    lib = _lib.get_lib()
+    t = DTYPES[x.dtype]
+    y = torch.empty_like(x)
+    n = lib._pgt_group_norm_ws_floats(B, S, C, groups, t, 0)
+    ws = stats = None
+    if n > 0:
+        ws = torch.empty(n, dtype=F32, device=x.device)
+    if keep and (S > 1 or C // groups > 512):
+        stats = torch.empty(B, groups, 2, dtype=F32, device=x.device)
+    _timed("group_norm", 2.0 * x.numel() * x.element_size() if KERNEL_TIMER else 0, lambda: lib.call(
+        "pgt_group_norm_act", x.data_ptr(), B, S, C, groups, t, ptr(weight), ptr(bias), eps, act, y.data_ptr(), ptr(stats), ptr(ws), n,
+        stream_of(lib, x)))
+    return y, stats
+
+
 class GroupNormActFunction(torch.autograd.Function):
-    """pgt_group_norm_act / pgt_group_norm_act_bwd on x [B, rows, C] contiguous."""
+    """pgt_group_norm_act / pgt_group_norm_act_bwd on x [B, .., C] contiguous."""
 
     @staticmethod
-    def forward(ctx, x, groups, weight, bias, eps, act):
-        lib = _lib.get_lib()
-        B, S, C = x.shape
-        t = DTYPES[x.dtype]
-        y = torch.empty_like(x)
-        stats = torch.empty(B, groups, 2, dtype=F32, device=x.device) if S > 1 or C // groups > 512 else None
-        n = int(lib._pgt_group_norm_ws_floats(B, S, C, groups, t, 0))
-        ws = torch.empty(n, dtype=F32, device=x.device) if n > 0 else None
-        _timed("group_norm", 2.0 * x.numel() * x.element_size() if KERNEL_TIMER else 0, lambda: lib.call(
-            "pgt_group_norm_act", ptr(x), B, S, C, groups, t, ptr(weight), ptr(bias), eps, act, ptr(y), ptr(stats), ptr(ws), n,
-            stream_of(lib, x)))
+    def forward(ctx, x, weight, bias, args):
+        y, stats = _forward(x, *args[:4], weight, bias, *args[4:], True)
         ctx.save_for_backward(x, weight, bias, stats)
-        ctx.args = (groups, eps, act)
+        ctx.args = args
         return y
 
     @staticmethod
@@ -38,19 +46,19 @@ class GroupNormActFunction(torch.autograd.Function):
     def backward(ctx, dy):
         lib = _lib.get_lib()
         x, weight, bias, stats = ctx.saved_tensors
-        groups, eps, act = ctx.args
-        B, S, C = x.shape
-        t = DTYPES[x.dtype]
+        B, S, C, groups, eps, act = ctx.args
+        t, dev = DTYPES[x.dtype], x.device
         dy = dy.contiguous()
-        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(C, dtype=F32, device=x.device) if weight is not None and ctx.needs_input_grad[2] else None
-        db = torch.empty(C, dtype=F32, device=x.device) if bias is not None and ctx.needs_input_grad[3] else None
-        n = int(lib._pgt_group_norm_ws_floats(B, S, C, groups, t, 1))
-        ws = torch.empty(n, dtype=F32, device=x.device) if n > 0 else None
+        need = ctx.needs_input_grad
+        dx = torch.empty_like(x) if need[0] else None
+        dw = torch.empty(C, dtype=F32, device=dev) if need[1] else None
+        db = torch.empty(C, dtype=F32, device=dev) if need[2] else None
+        n = lib._pgt_group_norm_ws_floats(B, S, C, groups, t, 1)
+        ws = torch.empty(n, dtype=F32, device=dev) if n > 0 else None
         _timed("group_norm_bwd", 3.0 * x.numel() * x.element_size() if KERNEL_TIMER else 0, lambda: lib.call(
-            "pgt_group_norm_act_bwd", ptr(x), ptr(dy), ptr(stats), B, S, C, groups, t, ptr(weight), ptr(bias), eps, act, ptr(dx), ptr(dw),
-            ptr(db), ptr(ws), n, stream_of(lib, x)))
-        return dx, None, dw, db, None, None
+            "pgt_group_norm_act_bwd", x.data_ptr(), dy.data_ptr(), ptr(stats), B, S, C, groups, t, ptr(weight), ptr(bias), eps, act,
+            ptr(dx), ptr(dw), ptr(db), ptr(ws), n, stream_of(lib, x)))
+        return dx, dw, db, None
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
@@ -82,8 +90,12 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation=N
     rows = 1
     for n in x.shape[1:-1]:
         rows *= n
-    with torch.cuda.device_of(x):
-        y = GroupNormActFunction.apply(x.contiguous().view(x.size(0), rows, C), num_groups,
-                                       weight.contiguous() if weight is not None else None,
-                                       bias.contiguous() if bias is not None else None, float(eps), ACTIVATIONS[activation])
-    return y.view(x.shape)
+    x = x.contiguous()
+    weight = weight.contiguous() if weight is not None else None
+    bias = bias.contiguous() if bias is not None else None
+    args = (x.size(0), rows, C, num_groups, float(eps), ACTIVATIONS[activation])
+    with on_device(x):
+        if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad
+                                        or bias is not None and bias.requires_grad):
+            return GroupNormActFunction.apply(x, weight, bias, args)
+        return _forward(x, *args[:4], weight, bias, *args[4:], False)[0]
