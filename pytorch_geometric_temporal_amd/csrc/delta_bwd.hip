@@ -31,7 +31,7 @@ struct BwdArgs {
   float* dg; float* dbeta;       // [B, T, N, H]
   float* d_start;                // [P, K, V] or null
   float* seg_end;                // [P, segs - 1, K, V]: the gradient of the state behind every segment but the last
-  int vec, vec_do, vec_e, vec_s; // q, k / d_o / e / states can be read four values at a time
+  int vec;                       // every row can be read four values at a time
 };
 
 // One team per sequence and segment, chunks from the last to the first.  A wavefront owns sixteen value columns of dS and, in the
@@ -42,26 +42,25 @@ struct BwdArgs {
 // Tiles named [j][i] hold row j, column i of the transposed tile: an A operand of the transposed product read along rows, of the
 // product itself read down columns.  Bound by the fp32 matrix pipe from K = 64 on (2 K + 22 MFMAs of 32 cycles a wavefront and chunk).
 // STATE: only the gradient of the state before the segment, from a zero gradient behind it (the last segment: from d_last).
-// FULL: K = V = D and every row can be read four values at a time.
-template <class IO, int D, bool STATE, bool FULL>
-__global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_kernel(BwdArgs a) {
+// VEC: every row can be read four values at a time; FULL: K = V = D besides.
+template <class IO, int D, bool STATE, bool FULL, bool VEC>
+__global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bwd_kernel(BwdArgs a) {
   using TM = Team<D>;
   constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, NT = D / 16;
   constexpr int W_KQ = NW > 1 ? 1 : 0, W_OE = NW > 2 ? 2 : NW - 1, W_DG = NW > 2 ? 3 : 0;     // who does what in part 1
   struct Lds {
     float k[16 * LD], q[16 * LD], o[16 * LD], e[STATE ? 4 : 16 * LD], y[STATE ? 4 : 16 * LD];
     float x[STATE ? 4 : D * LD];                           // dS, for the product that contracts over its columns
-    float inv[256], p[256];                                // A operands, four values a lane
-    float am[TILE], m1[STATE ? 4 : TILE];                  // [j][i]
-    float kk[STATE ? 4 : 256], qk[STATE ? 4 : 256], db[STATE ? 4 : 256];      // K K^T, Q K^T, D_ij beta_j (i > j), as [j][i] four values a lane
-    float ye[STATE ? 1 : NW][STATE ? 4 : TILE];            // dY E^T by wavefront, [j][i]
+    float lane4[NW == 1 ? 1 : STATE ? 2 : 5][NW == 1 ? 4 : 256];              // tiles handed from wavefront to wavefront, four values a lane
+    float m1[STATE ? 4 : TILE];                            // [j][i]
+    float ye[STATE ? 1 : NW][TILE];                        // dY E^T by wavefront, [j][i]; before that, in part 1, ye[0]: A^T
     float red[STATE ? 1 : NW][4][16];                      // row sums by wavefront: dbeta, z, w, <S0, dS>
     float hi[NW][16], lo[NW][16], enter[16], leave[16], beta[16], whole[4];
   };
   __shared__ __attribute__((aligned(16))) char smem[sizeof(Lds) * TM::TEAMS];
   const Shape& s = a.s;
   const int K = FULL ? D : s.K, V = FULL ? D : s.V;
-  const int tid = (int)threadIdx.x, team = PGT_UNIFORM(tid / TL), tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane = tid & 63, col = lane & 15, cg = lane >> 4;
+  const int tid = (int)threadIdx.x, team = PGT_UNIFORM(tid / TL), tl = tid % TL, w = PGT_UNIFORM(tl / 64), lane0 = tid & 63, lane = lane0, col = lane & 15, cg = lane >> 4;
   Lds& L = reinterpret_cast<Lds*>(smem)[team];
   const int64_t first = s.p0 + (int64_t)blockIdx.x * TM::TEAMS;
   const Seq sq = seq_of(s, first + team);
@@ -82,6 +81,11 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
     for (int t = 0; t < NT; ++t) S[t] = zero4();
     if (from && sq.live) load_state<NT, FULL>(S, from + (seg == s.segs - 1 ? sq.p : sq.p * (s.segs - 1) + seg) * K * V, K, V, n, cg);
   }
+  // Tiles one wavefront makes and all use: through LDS, or in registers where there is but one.  0: (I + A)^-T, 1: P^T (A operands);
+  // 2: K K^T, 3: Q K^T, 4: D_ij beta_j (i > j), row i = 4 cg + r, column j = col
+  gd_f4 own[5];
+  auto give = [&](int which, gd_f4 x) { if (NW == 1) own[which] = x; else put4(&L.lane4[which][4 * lane], x); };
+  auto take = [&](int which) { return NW == 1 ? own[which] : lds4(&L.lane4[which][4 * lane]); };
   const int tok = tl / QD, qd = 4 * (tl % QD);
   const int nqk = FULL ? 4 : K - qd, nvv = FULL ? 4 : V - qd;      // values of this lane's quads that exist
   const IO* kp = at<IO>(a.k, sq, kh) + (nqk > 0 ? qd : 0);
@@ -90,17 +94,17 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
   const IO* op = reinterpret_cast<const IO*>(a.d_o) + seq_h * V + (nvv > 0 ? qd : 0);
   const float* ep = a.e + seq_h * V + (nvv > 0 ? qd : 0);
   const int last = s.T - 1;
-  Quad<IO> nk = {}, nq = {}, no = {};
-  Quad<float> ne = {};
+  Quad<IO, VEC> nk = {}, nq = {}, no = {};
+  Quad<float, VEC> ne = {};
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
     int t = 16 * c + tok, tg = 16 * c + col;
     t = t < last ? t : last;
     tg = tg < last ? tg : last;
-    read4<FULL>(nk, kp + t * a.k.st, nqk, a.vec != 0);
-    read4<FULL>(nq, qp + t * a.q.st, nqk, a.vec != 0);
-    read4<FULL>(no, op + t * row_v, nvv, a.vec_do != 0);
-    if (!STATE) read4<FULL>(ne, ep + t * row_v, nvv, a.vec_e != 0);
+    read4(nk, kp + t * a.k.st, nqk);
+    read4(nq, qp + t * a.q.st, nqk);
+    read4(no, op + t * row_v, nvv);
+    if (!STATE) read4(ne, ep + t * row_v, nvv);
     ng = gp[tg * a.g.st];
     nb = bp[tg * a.beta.st];
   };
@@ -108,6 +112,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
   // X_ij = M1_ij q_i.k_j + M2_ij k_i.k_j left of the diagonal (row i = 4 cg + r, column j = col), which wavefront W_DG kept
   gd_f4 pre = zero4();
   auto finish = [&](int c) {
+    const int lane = fresh(lane0), col = lane & 15, cg = lane >> 4;
     float dbv = 0.f, z = 0.f, wj = 0.f, dot = 0.f;
 #pragma unroll
     for (int u = 0; u < NW; ++u) {
@@ -145,16 +150,17 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
   for (int c = ce - 1; c >= c0; --c) {
     {
       const bool in = 16 * c + tok < sq.len;
-      put4(&L.k[tok * LD + qd], unpack<FULL>(nk, in ? nqk : 0));
-      gd_f4 x = unpack<FULL>(nq, in ? nqk : 0);
+      put4(&L.k[tok * LD + qd], unpack(nk, in ? nqk : 0));
+      gd_f4 x = unpack(nq, in ? nqk : 0);
 #pragma unroll
       for (int r = 0; r < 4; ++r) x[r] *= s.scale;
       put4(&L.q[tok * LD + qd], x);
-      put4(&L.o[tok * LD + qd], unpack<FULL>(no, in ? nvv : 0));
-      if (!STATE) put4(&L.e[tok * LD + qd], unpack<FULL>(ne, in ? nvv : 0));
+      put4(&L.o[tok * LD + qd], unpack(no, in ? nvv : 0));
+      if (!STATE) put4(&L.e[tok * LD + qd], unpack(ne, in ? nvv : 0));
     }
     const bool here = 16 * c + col < sq.len;
     const float g = here ? ng : 0.f, b = here ? nb : 0.f;
+    PGT_SCHED_FENCE();
     if (c > c0) fetch(c - 1);
     gd_f4 s0[STATE ? 1 : NT];                             // S0, row = this lane's key column, along the values
     const float* from = c > 0 ? a.states + (sq.p * (s.chunks - 1) + c - 1) * K * V : a.start ? a.start + sq.p * K * V : nullptr;
@@ -162,25 +168,20 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
       const float* base = from ? from : a.e;
       const bool in = from && kin;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int at = 16 * t + 4 * cg, left = V - at;
-        if (FULL) {
-          s0[t] = lds4(base + (in ? n * V + at : 0));
-        } else if (a.vec_s) {
-          const gd_f4 x = lds4(base + (in && left > 0 ? n * V + at : 0));
-#pragma unroll
-          for (int r = 0; r < 4; ++r) s0[t][r] = in && left > 0 ? x[r] : 0.f;
+      for (int t = 0; t < NT; ++t) {                      // (what lies outside is masked when it is used)
+        const int at = 16 * t + 4 * cg, left = in ? V - at : 0;
+        if (VEC) {
+          s0[t] = lds4(base + (left > 0 ? n * V + at : 0));
         } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float x = base[in && r < left ? n * V + at + r : 0];
-            s0[t][r] = in && r < left ? x : 0.f;
-          }
+          for (int r = 0; r < 4; ++r) s0[t][r] = base[r < left ? n * V + at + r : 0];
         }
       }
     }
     team_sync<D>();
     // ---- part 1
+    {
+    const int lane = fresh(lane0), col = lane & 15, cg = lane >> 4;
     if (!STATE && w == W_DG && c < ce - 1) finish(c + 1);
     if (w == 0 || w == W_KQ || (!STATE && w == W_OE)) {
       const Decay d = chunk_decay(g);
@@ -206,8 +207,8 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
         gd_f4 p;
 #pragma unroll
         for (int r = 0; r < 4; ++r) p[r] = dec[r] * qk[r];
-        put4(&L.p[4 * lane], p);
-        if (!STATE) put4(&L.qk[4 * lane], qk);
+        give(1, p);
+        if (!STATE) give(3, qk);
       }
       if (!STATE && w == W_OE) {
         gd_f4 m;
@@ -228,17 +229,18 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
           db[r] = x * b;
         }
         if (!STATE) {
-          put4(&L.kk[4 * lane], kk);
-          put4(&L.db[4 * lane], db);
+          give(2, kk);
+          give(4, db);
         }
-        put4(&L.am[col * TS + 4 * cg], m);                // row j of A^T
+        put4(&L.ye[0][col * TS + 4 * cg], m);                // row j of A^T
         gd_wave_sync();
         float arow[16];
-        row16(&L.am[col * TS], arow);
+        row16(&L.ye[0][col * TS], arow);
         gd_f4 inv = unit_row(lane);
         solve_up<15>(arow, inv);
-        put4(&L.inv[4 * lane], inv);
+        give(0, inv);
       }
+    }
     }
     arrive(nk);
     arrive(nq);
@@ -248,6 +250,8 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
     arrive(nb);
     team_sync<D>();
     // ---- part 2
+    {
+    const int lane = fresh(lane0), col = lane & 15, cg = lane >> 4, n = 16 * w + col;
     const gd_f4 enter = lds4(&L.enter[4 * cg]), leave = lds4(&L.leave[4 * cg]), beta = lds4(&L.beta[4 * cg]);
     const float whole = L.enter[15];
     if (w == 0 && lane == 0) L.whole[0] = whole;
@@ -264,8 +268,9 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
         dout[r] = L.o[(4 * cg + r) * LD + n];
         du[r] *= leave[r];
       }
-      du = mma16(lds4(&L.p[4 * lane]), dout, du);
-      const gd_f4 dr = mma16(lds4(&L.inv[4 * lane]), du, zero4());
+      du = mma16(take(1), dout, du);
+      const gd_f4 dr = mma16(take(0), du, zero4());
+      PGT_SCHED_FENCE();
       gd_f4 dy, eo, ey;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -287,6 +292,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
         }
         S[t] = mma16(kt, ey, mma16(qt, eo, S[t]));
       }
+      PGT_SCHED_FENCE();
       if (!STATE) {
         float db[4];
 #pragma unroll
@@ -323,10 +329,16 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
       gd_wave_sync();                                     // dY E^T over this wavefront's sixteen value columns
       const gd_f4 z = mma16(lds4(&L.y[col * LD + 16 * w + 4 * cg]), lds4(&L.e[col * LD + 16 * w + 4 * cg]), zero4());
       put4(&L.ye[w][col * TS + 4 * cg], z);
+    }
+    }
+    if (!STATE) {
       team_sync<D>();
       // ---- part 3
+      const int lane = fresh(lane0), col = lane & 15, cg = lane >> 4, n = 16 * w + col;
+      const gd_f4 enter = lds4(&L.enter[4 * cg]), leave = lds4(&L.leave[4 * cg]), beta = lds4(&L.beta[4 * cg]);
+      PGT_SCHED_FENCE();
       if (w == W_DG) {
-        const gd_f4 b = lds4(&L.db[4 * lane]), qk = lds4(&L.qk[4 * lane]), kk = lds4(&L.kk[4 * lane]), m1 = lds4(&L.m1[col * TS + 4 * cg]);
+        const gd_f4 b = take(4), qk = take(3), kk = take(2), m1 = lds4(&L.m1[col * TS + 4 * cg]);
         gd_f4 ye = zero4();
 #pragma unroll
         for (int u = 0; u < NW; ++u) {
@@ -337,10 +349,17 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
 #pragma unroll
         for (int r = 0; r < 4; ++r) pre[r] = 4 * cg + r > col ? m1[r] * qk[r] - b[r] * kk[r] * ye[r] : 0.f;
       }
+      PGT_SCHED_FENCE();
       if (kcols) {
         gd_f4 aq = zero4(), ak = zero4(), al = zero4();
         float dot = 0.f;
         if (from) {
+          if (!FULL) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) s0[t][r] = kin && 16 * t + 4 * cg + r < V ? s0[t][r] : 0.f;
+          }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             if (t % 4 == 0) PGT_SCHED_FENCE();
@@ -370,17 +389,22 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
             m2[r] += L.ye[u][(4 * cg + r) * TS + col];
           }
         }
-        const gd_f4 bt = lds4(&L.db[4 * lane]);
+        const gd_f4 bt = take(4);
         const gd_f4 m1t = lds4(&L.m1[col * TS + 4 * cg]);
+        // entry (i = col, j = 4 cg + r) of D beta, where `bt` has (i = 4 cg + r, j = col): with lane 16 (col / 4) + 4 cg + r as value col % 4
+        auto mirror = [&](int r) {
+          const int from_lane = 16 * (col >> 2) + 4 * cg + r;
+          if (NW > 1) return L.lane4[NW > 1 ? 4 : 0][NW > 1 ? 4 * from_lane + (col & 3) : 0];
+          const float v0 = __shfl(bt[0], from_lane), v1 = __shfl(bt[1], from_lane), v2 = __shfl(bt[2], from_lane), v3 = __shfl(bt[3], from_lane);
+          return (col & 3) == 0 ? v0 : (col & 3) == 1 ? v1 : (col & 3) == 2 ? v2 : v3;
+        };
         gd_f4 kc, qc, m1;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           kc[r] = L.k[(4 * cg + r) * LD + n];
           qc[r] = L.q[(4 * cg + r) * LD + n];
           m1[r] = L.m1[(4 * cg + r) * TS + col];
-          // the entry (i = 4 cg + r, j = col) of D beta lies with lane 16 (i / 4) + j as value i % 4: as written for this lane; its mirror
-          // (i = col, j = 4 cg + r) with lane 16 (col / 4) + 4 cg + r as value col % 4
-          m2[r] = -(m2[r] * L.db[4 * (16 * (col >> 2) + 4 * cg + r) + (col & 3)]) - m2t[r] * bt[r];
+          m2[r] = -(m2[r] * mirror(r)) - m2t[r] * bt[r];
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -391,6 +415,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES) void delta_bwd_ke
           if (col == 0) { L.red[w][1][4 * cg + r] = z; L.red[w][2][4 * cg + r] = wj; }
           ak[r] += al[r];
         }
+        PGT_SCHED_FENCE();
         dot = sum16(dot);
         if (col == 0) L.red[w][3][cg] = dot;
         aq = mma16(m1, kc, aq);
@@ -465,7 +490,7 @@ __global__ __launch_bounds__(256) void delta_heads_kernel(const float* x, IO* y,
   y[i] = from_f32<IO>(acc);
 }
 
-template <class IO, int D, bool STATE, bool FULL> void go(const BwdArgs& a0, pgt_stream_t stream) {
+template <class IO, int D, bool STATE, bool FULL, bool VEC> void go(const BwdArgs& a0, pgt_stream_t stream) {
   using TM = Team<D>;
   BwdArgs a = a0;
   const int64_t most = (int64_t)1 << 21;
@@ -473,17 +498,17 @@ template <class IO, int D, bool STATE, bool FULL> void go(const BwdArgs& a0, pgt
     a.s.p0 = p0;
     const int64_t wgs = pgt_cdiv(a.s.P - p0, TM::TEAMS);
     const dim3 grid((unsigned)(wgs < most ? wgs : most), (unsigned)(STATE ? a.s.segs - 1 : a.s.segs));
-    PGT_LAUNCH((delta_bwd_kernel<IO, D, STATE, FULL>), grid, dim3(TM::THREADS), stream, a);
+    PGT_LAUNCH((delta_bwd_kernel<IO, D, STATE, FULL, VEC>), grid, dim3(TM::THREADS), stream, a);
   }
 }
 template <class IO, int D> int all(const BwdArgs& a, const float* seg_trans, pgt_stream_t stream) {
-  const bool full = a.vec && a.vec_do && a.vec_e && a.vec_s && a.s.K == D && a.s.V == D;
+  const bool full = a.vec && a.s.K == D && a.s.V == D;
   if (a.s.segs > 1) {
-    if (full) go<IO, D, true, true>(a, stream); else go<IO, D, true, false>(a, stream);
+    if (full) go<IO, D, true, true, true>(a, stream); else if (a.vec) go<IO, D, true, false, true>(a, stream); else go<IO, D, true, false, false>(a, stream);
     if (a.s.segs > 2)
       if (int e = pgt_delta_join_up(seg_trans, a.seg_end, a.s.P, a.s.segs, a.s.K, a.s.V, stream)) return e;
   }
-  if (full) go<IO, D, false, true>(a, stream); else go<IO, D, false, false>(a, stream);
+  if (full) go<IO, D, false, true, true>(a, stream); else if (a.vec) go<IO, D, false, false, true>(a, stream); else go<IO, D, false, false, false>(a, stream);
   return pgt_check_launch("pgt_gated_delta_bwd");
 }
 template <class IO> int by_width(const BwdArgs& a0, void* dq, void* dk, const float* seg_trans, pgt_stream_t stream) {
@@ -530,9 +555,7 @@ extern "C" int pgt_gated_delta_bwd(const pgt_delta_dims* d, const pgt_seq_view* 
   a.dq = a.s.rep > 1 ? (void*)head_ws : dq;
   a.dk = a.s.rep > 1 ? (void*)(head_ws + n) : dk;
   a.dv = dv; a.dg = dg; a.dbeta = dbeta; a.d_start = d_start; a.seg_end = seg_end;
-  a.vec_do = a.s.V % 4 == 0 && pgt_aligned(d_o, d->dtype == PGT_DT_F32 ? 16 : 8);
-  a.vec_e = a.s.V % 4 == 0 && pgt_aligned(e, 16);
-  a.vec_s = a.vec_e && pgt_aligned(states, 16) && pgt_aligned(start, 16);
+  a.vec = a.vec && a.s.V % 4 == 0 && pgt_aligned(d_o, d->dtype == PGT_DT_F32 ? 16 : 8) && pgt_aligned(e, 16) && pgt_aligned(states, 16) && pgt_aligned(start, 16);
   if (d->dtype == PGT_DT_F32) return by_width<float>(a, dq, dk, seg_trans, stream);
   if (d->dtype == PGT_DT_BF16) return by_width<bf16>(a, dq, dk, seg_trans, stream);
   return by_width<f16>(a, dq, dk, seg_trans, stream);

@@ -182,37 +182,43 @@ __device__ __forceinline__ Seq seq_of(const Shape& s, int64_t p) {
   q.len = q.live ? len : 0;
   return q;
 }
-// Four values of a row in registers as loaded: packed in the storage type until they are used.  Every load is issued, from a valid
-// address in any case (row and first value clamped by the caller): a branch around each load costs more than the load.  What is not
-// there is masked when the quad is unpacked: n is how many of the four values exist (FULL, vec: four or none).
-template <class IO> struct Quad { int2 x; };
-template <> struct Quad<float> { gd_f4 x; };
-template <bool FULL> __device__ __forceinline__ void read4(Quad<float>& q, const float* p, int n, bool vec) {
-  if (FULL || vec) { q.x = lds4(p); return; }
+// Four values of a row in registers as loaded: in the storage type (VEC: one load, packed) until they are used.  Every load is issued, from
+// a valid address in any case (row and first value clamped by the caller), and nothing is computed with it: a branch around a load, or
+// a mask right behind it, makes the compiler wait for it there.  What is not there is masked when the quad is unpacked: n is how many
+// of the four values exist (VEC: four or none).
+template <class IO, bool VEC> struct Quad { IO x[4]; };
+template <> struct Quad<float, true> { gd_f4 x; };
+template <class IO> struct Quad<IO, true> { int2 x; };
+template <class IO> __device__ __forceinline__ void read4(Quad<IO, false>& q, const IO* p, int n) {
   q.x[0] = p[0]; q.x[1] = p[n > 1 ? 1 : 0]; q.x[2] = p[n > 2 ? 2 : 0]; q.x[3] = p[n > 3 ? 3 : 0];
 }
-template <bool FULL, class IO> __device__ __forceinline__ void read4(Quad<IO>& q, const IO* p, int n, bool vec) {
-  if (FULL || vec) { q.x = *reinterpret_cast<const int2*>(p); return; }
-  q.x.x = (int)(p[0].u | ((uint32_t)p[n > 1 ? 1 : 0].u << 16));
-  q.x.y = (int)(p[n > 2 ? 2 : 0].u | ((uint32_t)p[n > 3 ? 3 : 0].u << 16));
-}
-template <bool FULL> __device__ __forceinline__ gd_f4 unpack(const Quad<float>& q, int n) {
+__device__ __forceinline__ void read4(Quad<float, true>& q, const float* p, int) { q.x = lds4(p); }
+template <class IO> __device__ __forceinline__ void read4(Quad<IO, true>& q, const IO* p, int) { q.x = *reinterpret_cast<const int2*>(p); }
+template <class IO> __device__ __forceinline__ gd_f4 unpack(const Quad<IO, false>& q, int n) {
   gd_f4 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = n > (FULL ? 0 : i) ? q.x[i] : 0.f;
+  for (int i = 0; i < 4; ++i) r[i] = n > i ? to_f32(q.x[i]) : 0.f;
   return r;
 }
-template <bool FULL, class IO> __device__ __forceinline__ gd_f4 unpack(const Quad<IO>& q, int n) {
-  const uint32_t lo = n > 0 ? (uint32_t)q.x.x : 0u, hi = n > (FULL ? 0 : 2) ? (uint32_t)q.x.y : 0u;
+__device__ __forceinline__ gd_f4 unpack(const Quad<float, true>& q, int n) {
+  gd_f4 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = n > 0 ? q.x[i] : 0.f;
+  return r;
+}
+template <class IO> __device__ __forceinline__ gd_f4 unpack(const Quad<IO, true>& q, int n) {
+  const uint32_t lo = n > 0 ? (uint32_t)q.x.x : 0u, hi = n > 0 ? (uint32_t)q.x.y : 0u;
   gd_f4 r;
   r[0] = to_f32(IO{(uint16_t)(lo & 0xffffu)}); r[1] = to_f32(IO{(uint16_t)(lo >> 16)});
   r[2] = to_f32(IO{(uint16_t)(hi & 0xffffu)}); r[3] = to_f32(IO{(uint16_t)(hi >> 16)});
-  if (!FULL) {
-    if (n < 2) r[1] = 0.f;
-    if (n < 4) r[3] = 0.f;
-  }
   return r;
 }
+// The same number as far as the compiler cannot see: what is derived from it is computed again instead of kept in a register through a loop.
+#ifdef PGT_EMU
+inline int fresh(int x) { return x; }
+#else
+__device__ __forceinline__ int fresh(int x) { asm volatile("" : "+v"(x)); return x; }
+#endif
 // Waits for a load here.  A load that is used behind stores whose number the compiler cannot know would wait for the stores as well.
 #ifdef PGT_EMU
 template <class T> inline void arrive(T&) {}
@@ -220,8 +226,9 @@ template <class T> inline void arrive(T&) {}
 __device__ __forceinline__ void arrive(float& x) { asm volatile("" : "+v"(x)); }
 __device__ __forceinline__ void arrive(bf16& x) { uint32_t t = x.u; asm volatile("" : "+v"(t)); x.u = (uint16_t)t; }
 __device__ __forceinline__ void arrive(f16& x) { uint32_t t = x.u; asm volatile("" : "+v"(t)); x.u = (uint16_t)t; }
-__device__ __forceinline__ void arrive(Quad<float>& q) { asm volatile("" : "+v"(q.x)); }
-template <class IO> __device__ __forceinline__ void arrive(Quad<IO>& q) { asm volatile("" : "+v"(q.x.x), "+v"(q.x.y)); }
+__device__ __forceinline__ void arrive(Quad<float, true>& q) { asm volatile("" : "+v"(q.x)); }
+template <class IO> __device__ __forceinline__ void arrive(Quad<IO, true>& q) { asm volatile("" : "+v"(q.x.x), "+v"(q.x.y)); }
+template <class IO> __device__ __forceinline__ void arrive(Quad<IO, false>& q) { for (int i = 0; i < 4; ++i) arrive(q.x[i]); }
 #endif
 template <class T> __device__ __forceinline__ const T* at(const View& v, const Seq& q, int h) {
   return reinterpret_cast<const T*>(v.p) + (int64_t)q.b * v.sb + (int64_t)q.n * v.sn + (int64_t)h * v.sh;
@@ -245,6 +252,7 @@ template <int D> struct Team {             // a team of wavefronts owns a sequen
   static constexpr int TL = 64 * NW;
   static constexpr int THREADS = TL * TEAMS;
   static constexpr int WAVES = D == 16 ? 4 : D == 32 ? 3 : 2;      // wavefronts a SIMD that the register allocation makes room for
+  static constexpr int WAVES_BWD = D <= 32 ? 3 : 2;
   static constexpr int LD = D + 4;         // LDS row stride: rows of sixteen lanes x 16 bytes cover the banks once
   static constexpr int SB = D == 128 ? 4 : NW;              // chunks the forward kernel prepares side by side
 };

@@ -25,8 +25,8 @@ struct FwdArgs {
 // pipe's rate: what bounds it at K = 64 and beyond; narrow heads are bound by memory and by the preparation's vector instructions.
 // TRANS: what a long sequence with few heads is split with: blockIdx.z 0: only the state behind the segment, from a zero start (the
 // first segment: from the sequence's); 1: the segment's transition matrix, i.e. the same recurrence with v = 0 from the unit matrix.
-// FULL: K = V = D and rows can be read four values at a time.
-template <class IO, int D, bool TRANS, bool FULL>
+// VEC: rows can be read four values at a time; FULL: K = V = D besides.
+template <class IO, int D, bool TRANS, bool FULL, bool VEC>
 __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void delta_fwd_kernel(FwdArgs a) {
   using TM = Team<D>;
   constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, SB = TM::SB, TB = 16 * SB, NT = D / 16;
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
   const IO* qp = at<IO>(a.q, sq, kh) + (nqk > 0 ? qd : 0);
   const IO* vp = at<IO>(a.v, sq, sq.h) + (vin ? n : 0);
   const int last = s.T - 1;
-  Quad<IO> nk[SB] = {}, nq[TRANS ? 1 : SB] = {};
+  Quad<IO, VEC> nk[SB] = {}, nq[TRANS ? 1 : SB] = {};
   IO nv[SB][4] = {};
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
@@ -82,8 +82,8 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
     for (int i = 0; i < SB; ++i) {
       int t = 16 * (c + i) + tok;
       t = t < last ? t : last;
-      read4<FULL>(nk[i], kp + t * a.k.st, nqk, a.vec != 0);
-      if (!TRANS) read4<FULL>(nq[i], qp + t * a.q.st, nqk, a.vec != 0);
+      read4(nk[i], kp + t * a.k.st, nqk);
+      if (!TRANS) read4(nq[i], qp + t * a.q.st, nqk);
     }
     int tg = 16 * (c + (SB < NW ? w % SB : w)) + col;
     tg = tg < last ? tg : last;
@@ -107,9 +107,9 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
       const int have = 16 * (c + i) + tok < sq.len ? nqk : 0;
-      put4(&L.k[(16 * i + tok) * LD + qd], unpack<FULL>(nk[i], have));
+      put4(&L.k[(16 * i + tok) * LD + qd], unpack(nk[i], have));
       if (!TRANS) {
-        gd_f4 x = unpack<FULL>(nq[i], have);
+        gd_f4 x = unpack(nq[i], have);
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] *= s.scale;
         put4(&L.q[(16 * i + tok) * LD + qd], x);
@@ -263,8 +263,8 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
 // x [P, segs - 1, K, V] holds the second summand and takes the sum (its entry 0 is complete already).  UP (the adjoint): from the last
 // entry down with the transposed transitions.  A workgroup owns sixteen columns of a sequence's state, a wavefront sixteen rows; the
 // next two transitions are on their way while one is multiplied: what remains of a step is its K / 4 dependent MFMAs and one barrier.
-template <int D, bool UP>
-__global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K, int V, int vec) {
+template <int D, bool UP, bool VEC>
+__global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K, int V) {
   constexpr int LD = D + 4, NT = D / 16;
   __shared__ __attribute__((aligned(16))) float st[2][16 * LD];     // [column][row], two buffers
   const int w = (int)threadIdx.x / 64, lane = (int)threadIdx.x & 63, col = lane & 15, cg = lane >> 4;
@@ -279,33 +279,27 @@ __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* 
   auto fetch = [&](int j, gd_f4 (&m)[NT], gd_f4& add) {                               // step j: entry `to` takes the transition of segment `tr`
     const int to = UP ? entries - 1 - j : j, tr = UP ? entries - j : j;
     const float* q = mp + (int64_t)(tr - 1) * K * K;
+    // (what lies outside the matrix is its first value: it only meets state rows that are zero, and rows that are not kept)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {                        // (elements outside: the matrix's own first value, masked)
+    for (int t = 0; t < NT; ++t) {
       const int left = i < K ? K - 16 * t - 4 * cg : 0;
-      if (!UP && vec) {
-        const gd_f4 x = lds4(q + (left > 0 ? at_m + 16 * t : 0));
-#pragma unroll
-        for (int r = 0; r < 4; ++r) m[t][r] = left > 0 ? x[r] : 0.f;
+      if (VEC) {
+        m[t] = lds4(q + (left > 0 ? at_m + 16 * t : 0));
       } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float x = q[r < left ? (UP ? at_m + (16 * t + r) * K : at_m + 16 * t + r) : 0];
-          m[t][r] = r < left ? x : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) m[t][r] = q[r < left ? (UP ? at_m + (16 * t + r) * K : at_m + 16 * t + r) : 0];
       }
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool in = row0 + r < K && n < V;
-      const float x = x0[(int64_t)to * K * V + (in ? (row0 + r) * V + n : 0)];
-      add[r] = in ? x : 0.f;
-    }
+    for (int r = 0; r < 4; ++r) add[r] = x0[(int64_t)to * K * V + (row0 + r < K && n < V ? (row0 + r) * V + n : 0)];
   };
   gd_f4 s;
 #pragma unroll
   for (int r = 0; r < 4; ++r) s[r] = row0 + r < K && n < V ? xp[((int64_t)(UP ? entries - 1 : 0) * K + r) * V] : 0.f;
   auto step = [&](int j, gd_f4 (&m)[NT], gd_f4& add) {
     float* buf = st[j & 1];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = row0 + r < K ? s[r] : 0.f;
     put4(&buf[col * LD + row0], s);
     gd_block_sync();
     s = add;
@@ -327,7 +321,7 @@ __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* 
   if (j < entries) step(j, m0, add0);
 }
 
-template <class IO, int D, bool TRANS, bool FULL> void go(const FwdArgs& a0, pgt_stream_t stream) {
+template <class IO, int D, bool TRANS, bool FULL, bool VEC> void go(const FwdArgs& a0, pgt_stream_t stream) {
   using TM = Team<D>;
   FwdArgs a = a0;
   const int64_t most = (int64_t)1 << 21;                  // workgroups of a launch: the grid's threads stay below 2^32
@@ -335,19 +329,22 @@ template <class IO, int D, bool TRANS, bool FULL> void go(const FwdArgs& a0, pgt
     a.s.p0 = p0;
     const int64_t wgs = pgt_cdiv(a.s.P - p0, TM::TEAMS);
     const dim3 grid((unsigned)(wgs < most ? wgs : most), (unsigned)(TRANS ? a.s.segs - 1 : a.s.segs), TRANS && a.s.segs > 2 ? 2 : 1);
-    PGT_LAUNCH((delta_fwd_kernel<IO, D, TRANS, FULL>), grid, dim3(TM::THREADS), stream, a);
+    PGT_LAUNCH((delta_fwd_kernel<IO, D, TRANS, FULL, VEC>), grid, dim3(TM::THREADS), stream, a);
   }
+}
+template <int D, bool UP> void join(const float* trans, float* x, int64_t P, int segs, int K, int V, pgt_stream_t stream) {
+  const dim3 grid((unsigned)P, (unsigned)((V + 15) / 16)), block(64 * (D / 16));
+  if (!UP && K % 4 == 0 && pgt_aligned(trans, 16)) PGT_LAUNCH((delta_join_kernel<D, UP, !UP>), grid, block, stream, trans, x, segs, K, V);
+  else PGT_LAUNCH((delta_join_kernel<D, UP, false>), grid, block, stream, trans, x, segs, K, V);
 }
 template <class IO, int D> void all(const FwdArgs& a, pgt_stream_t stream) {
   const bool full = a.vec && a.s.K == D && a.s.V == D;
   if (a.s.segs > 1) {
-    if (full) go<IO, D, true, true>(a, stream); else go<IO, D, true, false>(a, stream);
-    if (a.s.segs > 2) {
-      const dim3 grid((unsigned)a.s.P, (unsigned)((a.s.V + 15) / 16));
-      PGT_LAUNCH((delta_join_kernel<D, false>), grid, dim3(64 * (D / 16)), stream, (const float*)a.seg_trans, a.seg_start, a.s.segs, a.s.K, a.s.V, (int)(a.s.K % 4 == 0 && pgt_aligned(a.seg_trans, 16)));
-    }
+    if (full) go<IO, D, true, true, true>(a, stream); else if (a.vec) go<IO, D, true, false, true>(a, stream); else go<IO, D, true, false, false>(a, stream);
+    if (a.s.segs > 2)
+      join<D, false>(a.seg_trans, a.seg_start, a.s.P, a.s.segs, a.s.K, a.s.V, stream);
   }
-  if (full) go<IO, D, false, true>(a, stream); else go<IO, D, false, false>(a, stream);
+  if (full) go<IO, D, false, true, true>(a, stream); else if (a.vec) go<IO, D, false, false, true>(a, stream); else go<IO, D, false, false, false>(a, stream);
 }
 template <class IO> void by_width(const FwdArgs& a, pgt_stream_t stream) {
   const int d = a.s.K > a.s.V ? a.s.K : a.s.V;
@@ -360,12 +357,11 @@ template <class IO> void by_width(const FwdArgs& a, pgt_stream_t stream) {
 }  // namespace
 
 int pgt_delta_join_up(const float* trans, float* x, int64_t P, int segs, int K, int V, pgt_stream_t stream) {
-  const dim3 grid((unsigned)P, (unsigned)((V + 15) / 16));
   const int d = K > V ? K : V;
-  if (d <= 16) PGT_LAUNCH((delta_join_kernel<16, true>), grid, dim3(64), stream, trans, x, segs, K, V, 0);
-  else if (d <= 32) PGT_LAUNCH((delta_join_kernel<32, true>), grid, dim3(128), stream, trans, x, segs, K, V, 0);
-  else if (d <= 64) PGT_LAUNCH((delta_join_kernel<64, true>), grid, dim3(256), stream, trans, x, segs, K, V, 0);
-  else PGT_LAUNCH((delta_join_kernel<128, true>), grid, dim3(512), stream, trans, x, segs, K, V, 0);
+  if (d <= 16) join<16, true>(trans, x, P, segs, K, V, stream);
+  else if (d <= 32) join<32, true>(trans, x, P, segs, K, V, stream);
+  else if (d <= 64) join<64, true>(trans, x, P, segs, K, V, stream);
+  else join<128, true>(trans, x, P, segs, K, V, stream);
   return pgt_check_launch("pgt_gated_delta_bwd");
 }
 
