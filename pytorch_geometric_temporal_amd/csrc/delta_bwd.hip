@@ -53,7 +53,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
     float x[STATE ? 4 : D * LD];                           // dS, for the product that contracts over its columns
     float lane4[NW == 1 ? 1 : STATE ? 2 : 5][NW == 1 ? 4 : 256];              // tiles handed from wavefront to wavefront, four values a lane
     float m1[STATE ? 4 : TILE];                            // [j][i]
-    float ye[STATE ? 1 : NW][TILE];                        // dY E^T by wavefront, [j][i]; before that, in part 1, ye[0]: A^T
+    float ye[STATE ? 1 : NW][TILE];                        // dY E^T by wavefront, [j][i]; before that, in part 1, ye[0]: -A^T
     float red[STATE ? 1 : NW][4][16];                      // row sums by wavefront: dbeta, z, w, <S0, dS>
     float hi[NW][16], lo[NW][16], enter[16], leave[16], beta[16], whole[4];
   };
@@ -88,25 +88,41 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
   auto take = [&](int which) { return NW == 1 ? own[which] : lds4(&L.lane4[which][4 * lane]); };
   const int tok = tl / QD, qd = 4 * (tl % QD);
   const int nqk = FULL ? 4 : K - qd, nvv = FULL ? 4 : V - qd;      // values of this lane's quads that exist
-  const IO* kp = at<IO>(a.k, sq, kh) + (nqk > 0 ? qd : 0);
-  const IO* qp = at<IO>(a.q, sq, kh) + (nqk > 0 ? qd : 0);
+  const IO* kp = at<IO>(a.k, sq, kh);
+  const IO* qp = at<IO>(a.q, sq, kh);
   const int64_t row_v = row_h * V;
-  const IO* op = reinterpret_cast<const IO*>(a.d_o) + seq_h * V + (nvv > 0 ? qd : 0);
-  const float* ep = a.e + seq_h * V + (nvv > 0 ? qd : 0);
-  const int last = s.T - 1;
+  const IO* op = reinterpret_cast<const IO*>(a.d_o) + seq_h * V;
+  const float* ep = a.e + seq_h * V;
+  const int qc = nqk > 0 ? qd : 0, vc = nvv > 0 ? qd : 0;
+  constexpr int ES = (int)sizeof(IO);
+  const uint32_t k_off = (uint32_t)(tok * (int)a.k.st + qc) * ES, q_off = (uint32_t)(tok * (int)a.q.st + qc) * ES;
+  const uint32_t v_off = (uint32_t)(tok * (int)row_v + vc), g_off = (uint32_t)(col * (int)a.g.st) * 4, b_off = (uint32_t)(col * (int)a.beta.st) * 4;
   Quad<IO, VEC> nk = {}, nq = {}, no = {};
   Quad<float, VEC> ne = {};
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
-    int t = 16 * c + tok, tg = 16 * c + col;
-    t = t < last ? t : last;
-    tg = tg < last ? tg : last;
-    read4(nk, kp + t * a.k.st, nqk);
-    read4(nq, qp + t * a.q.st, nqk);
-    read4(no, op + t * row_v, nvv);
-    if (!STATE) read4(ne, ep + t * row_v, nvv);
-    ng = gp[tg * a.g.st];
-    nb = bp[tg * a.beta.st];
+    const int64_t t0 = 16 * c;
+    const int left = s.T - 1 - 16 * c;
+    const IO* kb = kp + t0 * a.k.st;
+    const IO* qb = qp + t0 * a.q.st;
+    const float* gb = gp + t0 * a.g.st;
+    const float* bb = bp + t0 * a.beta.st;
+    if (left >= 15) {
+      read4(nk, by(kb, k_off), nqk);
+      read4(nq, by(qb, q_off), nqk);
+      read4(no, by(op + t0 * row_v, v_off * ES), nvv);
+      if (!STATE) read4(ne, by(ep + t0 * row_v, v_off * 4), nvv);
+      ng = *by(gb, g_off);
+      nb = *by(bb, b_off);
+    } else {                                              // rows behind the tensor: its last one, masked when used
+      const int t = tok < left ? tok : left, tg = col < left ? col : left;
+      read4(nk, by(kb, (uint32_t)(t * (int)a.k.st + qc) * ES), nqk);
+      read4(nq, by(qb, (uint32_t)(t * (int)a.q.st + qc) * ES), nqk);
+      read4(no, by(op + t0 * row_v, (uint32_t)(t * (int)row_v + vc) * ES), nvv);
+      if (!STATE) read4(ne, by(ep + t0 * row_v, (uint32_t)(t * (int)row_v + vc) * 4), nvv);
+      ng = *by(gb, (uint32_t)(tg * (int)a.g.st) * 4);
+      nb = *by(bb, (uint32_t)(tg * (int)a.beta.st) * 4);
+    }
   };
   // dg and dbeta of chunk c, while the next one's tiles are made, from the row sums in LDS and
   // X_ij = M1_ij q_i.k_j + M2_ij k_i.k_j left of the diagonal (row i = 4 cg + r, column j = col), which wavefront W_DG kept
@@ -225,19 +241,19 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float x = 4 * cg + r > col ? (NW > 2 || STATE ? dec[r] : gd_exp2((hi[r] - d.hi) + (li[r] - d.lo))) : 0.f;
-          m[r] = bi[r] * x * kk[r];
+          m[r] = -(bi[r] * x * kk[r]);
           db[r] = x * b;
         }
         if (!STATE) {
           give(2, kk);
           give(4, db);
         }
-        put4(&L.ye[0][col * TS + 4 * cg], m);                // row j of A^T
+        put4(&L.ye[0][col * TS + 4 * cg], m);                // row j of -A^T
         gd_wave_sync();
         float arow[16];
         row16(&L.ye[0][col * TS], arow);
         gd_f4 inv = unit_row(lane);
-        solve_up<15>(arow, inv);
+        solve_up(arow, inv);
         give(0, inv);
       }
     }
@@ -302,15 +318,16 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
           for (int r = 0; r < 4; ++r) L.red[w][0][4 * cg + r] = db[r];
         }
         if (sq.live && vin) {
-          const int64_t at = (seq_h + (int64_t)(16 * c + 4 * cg) * row_h) * V + n;
-          const int left = 16 * c + 16 <= s.T ? 4 : s.T - 16 * c - 4 * cg;
-          if (left >= 4) {
+          IO* to = reinterpret_cast<IO*>(a.dv) + (seq_h + (int64_t)(16 * c) * row_h) * V;
+          const uint32_t off = (uint32_t)(4 * cg * (int)row_v + n) * ES;
+          if (16 * c + 16 <= s.T) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) reinterpret_cast<IO*>(a.dv)[at + r * row_v] = from_f32<IO>(dy[r]);
+            for (int r = 0; r < 4; ++r) *by(to + r * row_v, off) = from_f32<IO>(dy[r]);
           } else {
+            const int left = s.T - 16 * c - 4 * cg;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (r < left) reinterpret_cast<IO*>(a.dv)[at + r * row_v] = from_f32<IO>(dy[r]);
+              if (r < left) *by(to + r * row_v, off) = from_f32<IO>(dy[r]);
           }
         }
       }
@@ -424,11 +441,12 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
         if (sq.live && kin) {
           const int left = s.T - 16 * c - 4 * cg;
           const int64_t row_k = (s.rep > 1 ? row_h : (int64_t)s.N * (s.H / s.rep)) * K;
-          const int64_t at = (s.rep > 1 ? seq_h : ((int64_t)sq.b * s.T * s.N + sq.n) * (s.H / s.rep) + kh) * K + (int64_t)(16 * c + 4 * cg) * row_k + n;
+          const int64_t at = (s.rep > 1 ? seq_h : ((int64_t)sq.b * s.T * s.N + sq.n) * (s.H / s.rep) + kh) * K + (int64_t)(16 * c) * row_k;
+          const uint32_t off = (uint32_t)(4 * cg * (int)row_k + n);
           auto put = [&](auto* dq, auto* dk, int r) {
             using T = std::remove_pointer_t<decltype(dq)>;
-            dq[at + r * row_k] = from_f32<T>(aq[r] * s.scale);
-            dk[at + r * row_k] = from_f32<T>(ak[r]);
+            *by(dq + at + r * row_k, off * (uint32_t)sizeof(T)) = from_f32<T>(aq[r] * s.scale);
+            *by(dk + at + r * row_k, off * (uint32_t)sizeof(T)) = from_f32<T>(ak[r]);
           };
           auto rows = [&](auto* dq, auto* dk) {
             if (16 * c + 16 <= s.T) {
@@ -540,6 +558,11 @@ extern "C" int pgt_gated_delta_bwd(const pgt_delta_dims* d, const pgt_seq_view* 
   if (a.s.T > 0) {
     PGT_REQUIRE(q && k && g && beta && q->data && k->data && g->data && beta->data && e && d_o && dq && dk && dv && dg && dbeta,
                 "pgt_gated_delta_bwd: null pointer");
+    const int es = d->dtype == PGT_DT_F32 ? 4 : 2;
+    PGT_REQUIRE(pgt_delta_near(d, q, es) && pgt_delta_near(d, k, es) && pgt_delta_near(d, g, 4) && pgt_delta_near(d, beta, 4),
+                "pgt_gated_delta_bwd: a step's stride is negative or above 2^27 bytes");
+    PGT_REQUIRE(d->nodes * d->heads * d->value < ((int64_t)1 << 25) - 128 && d->nodes * d->heads * d->key < ((int64_t)1 << 25) - 128,
+                "pgt_gated_delta_bwd: more than 2^25 values a step and sample");
     PGT_REQUIRE(a.s.chunks == 1 || states, "pgt_gated_delta_bwd: %d chunks need the forward pass's states", a.s.chunks);
     a.q = pgt_delta_view(q); a.k = pgt_delta_view(k); a.g = pgt_delta_view(g); a.beta = pgt_delta_view(beta);
     a.vec = pgt_delta_vec(q, a.s.K, d->dtype) && pgt_delta_vec(k, a.s.K, d->dtype);

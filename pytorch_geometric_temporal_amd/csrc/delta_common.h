@@ -101,23 +101,52 @@ __device__ __forceinline__ float sum16(float x) {       // the sum over the row 
   x += gd_ror16<1>(x);
   return x;
 }
-// X = (I + A)^-1 for A strictly lower triangular, lane l holding row i = l % 16 of A in a[] and X[i][4 (l / 16) + c] in t[c] (at first the
+// X = (I - A)^-1 for A strictly lower triangular, lane l holding row i = l % 16 of A in a[] and X[i][4 (l / 16) + c] in t[c] (at first the
 // unit matrix).  Forward substitution, one broadcast row a step: backward stable, no powers of A.  a[j] is 0 for j >= i.
-template <int J> __device__ __forceinline__ void solve_down(const float (&a)[16], gd_f4& t) {
+// (solve_up: strictly upper triangular, from the last row up; a[j] is 0 for j <= i.)
+// On the device the sixty updates are one block of v_fmac_f32_dpp (the compiler leaves a move before each fma): a row's value is
+// written three instructions before the next step broadcasts it, more than the two the hardware asks for; s_nop covers the first.
+#ifdef PGT_EMU
+template <int J> inline void solve_down(const float (&a)[16], gd_f4& t) {
   if constexpr (J < 15) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) t[c] = fmaf(-a[J], gd_bcast16<J>(t[c]), t[c]);
+    for (int c = 0; c < 4; ++c) t[c] = fmaf(gd_bcast16<J>(t[c]), a[J], t[c]);
     solve_down<J + 1>(a, t);
   }
 }
-// the same for A strictly upper triangular, from the last row up; a[j] is 0 for j <= i
-template <int J> __device__ __forceinline__ void solve_up(const float (&a)[16], gd_f4& t) {
+template <int J> inline void solve_up(const float (&a)[16], gd_f4& t) {
   if constexpr (J > 0) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) t[c] = fmaf(-a[J], gd_bcast16<J>(t[c]), t[c]);
+    for (int c = 0; c < 4; ++c) t[c] = fmaf(gd_bcast16<J>(t[c]), a[J], t[c]);
     solve_up<J - 1>(a, t);
   }
 }
+inline void solve_down(const float (&a)[16], gd_f4& t) { solve_down<0>(a, t); }
+inline void solve_up(const float (&a)[16], gd_f4& t) { solve_up<15>(a, t); }
+#else
+#define GD_ROW(J, N)                                                              \
+  "v_fmac_f32_dpp %0, %0, %" #N " row_newbcast:" #J " row_mask:0xf bank_mask:0xf\n\t" \
+  "v_fmac_f32_dpp %1, %1, %" #N " row_newbcast:" #J " row_mask:0xf bank_mask:0xf\n\t" \
+  "v_fmac_f32_dpp %2, %2, %" #N " row_newbcast:" #J " row_mask:0xf bank_mask:0xf\n\t" \
+  "v_fmac_f32_dpp %3, %3, %" #N " row_newbcast:" #J " row_mask:0xf bank_mask:0xf\n\t"
+__device__ __forceinline__ void solve_down(const float (&a)[16], gd_f4& t) {
+  float x = t[0], y = t[1], z = t[2], w = t[3];
+  asm("s_nop 1\n\t" GD_ROW(0, 4) GD_ROW(1, 5) GD_ROW(2, 6) GD_ROW(3, 7) GD_ROW(4, 8) GD_ROW(5, 9) GD_ROW(6, 10) GD_ROW(7, 11) GD_ROW(8, 12)
+      GD_ROW(9, 13) GD_ROW(10, 14) GD_ROW(11, 15) GD_ROW(12, 16) GD_ROW(13, 17) GD_ROW(14, 18) "s_nop 1"
+      : "+v"(x), "+v"(y), "+v"(z), "+v"(w)
+      : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "v"(a[8]), "v"(a[9]), "v"(a[10]), "v"(a[11]),
+        "v"(a[12]), "v"(a[13]), "v"(a[14]));
+  t[0] = x; t[1] = y; t[2] = z; t[3] = w;
+}
+__device__ __forceinline__ void solve_up(const float (&a)[16], gd_f4& t) {
+  float x = t[0], y = t[1], z = t[2], w = t[3];
+  asm("s_nop 1\n\t" GD_ROW(15, 4) GD_ROW(14, 5) GD_ROW(13, 6) GD_ROW(12, 7) GD_ROW(11, 8) GD_ROW(10, 9) GD_ROW(9, 10) GD_ROW(8, 11) GD_ROW(7, 12)
+      GD_ROW(6, 13) GD_ROW(5, 14) GD_ROW(4, 15) GD_ROW(3, 16) GD_ROW(2, 17) GD_ROW(1, 18) "s_nop 1"
+      : "+v"(x), "+v"(y), "+v"(z), "+v"(w)
+      : "v"(a[15]), "v"(a[14]), "v"(a[13]), "v"(a[12]), "v"(a[11]), "v"(a[10]), "v"(a[9]), "v"(a[8]), "v"(a[7]), "v"(a[6]), "v"(a[5]), "v"(a[4]),
+        "v"(a[3]), "v"(a[2]), "v"(a[1]));
+  t[0] = x; t[1] = y; t[2] = z; t[3] = w;
+}
+#undef GD_ROW
+#endif
 __device__ __forceinline__ gd_f4 unit_row(int lane) {
   gd_f4 t;
 #pragma unroll
@@ -230,6 +259,9 @@ __device__ __forceinline__ void arrive(Quad<float, true>& q) { asm volatile("" :
 template <class IO> __device__ __forceinline__ void arrive(Quad<IO, true>& q) { asm volatile("" : "+v"(q.x.x), "+v"(q.x.y)); }
 template <class IO> __device__ __forceinline__ void arrive(Quad<IO, false>& q) { for (int i = 0; i < 4; ++i) arrive(q.x[i]); }
 #endif
+// p (the same in every lane) and a lane's own offset in bytes: one scalar base and one register, no 64-bit sum a lane
+template <class T> __device__ __forceinline__ const T* by(const T* p, uint32_t bytes) { return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + bytes); }
+template <class T> __device__ __forceinline__ T* by(T* p, uint32_t bytes) { return reinterpret_cast<T*>(reinterpret_cast<char*>(p) + bytes); }
 template <class T> __device__ __forceinline__ const T* at(const View& v, const Seq& q, int h) {
   return reinterpret_cast<const T*>(v.p) + (int64_t)q.b * v.sb + (int64_t)q.n * v.sn + (int64_t)h * v.sh;
 }
@@ -287,5 +319,6 @@ template <int D> __device__ __forceinline__ void team_sync() {
 // host side (delta_fwd.hip): the checked shape with its plan, views, whether rows can be read four values at a time, the adjoint's join
 int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s);
 gd::View pgt_delta_view(const pgt_seq_view* v);
+bool pgt_delta_near(const pgt_delta_dims* d, const pgt_seq_view* v, int size);
 bool pgt_delta_vec(const pgt_seq_view* v, int width, int dtype);
 int pgt_delta_join_up(const float* trans, float* x, int64_t P, int segs, int K, int V, pgt_stream_t stream);

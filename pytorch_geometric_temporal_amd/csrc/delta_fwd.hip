@@ -70,38 +70,55 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
   // what the next block brings, in registers: SB quads of k and q a lane, the wavefront's own column of v, the decays of one chunk
   const int tok = tl / QD, qd = 4 * (tl % QD);
   const int nqk = FULL ? 4 : K - qd;                      // values of this lane's quad that exist
-  const IO* kp = at<IO>(a.k, sq, kh) + (nqk > 0 ? qd : 0);
-  const IO* qp = at<IO>(a.q, sq, kh) + (nqk > 0 ? qd : 0);
-  const IO* vp = at<IO>(a.v, sq, sq.h) + (vin ? n : 0);
-  const int last = s.T - 1;
+  const IO* kp = at<IO>(a.k, sq, kh);
+  const IO* qp = at<IO>(a.q, sq, kh);
+  const IO* vp = at<IO>(a.v, sq, sq.h);
+  const int qc = nqk > 0 ? qd : 0, vc = vin ? n : 0;
+  constexpr int ES = (int)sizeof(IO);
+  const uint32_t k_off = (uint32_t)(tok * (int)a.k.st + qc) * ES, q_off = (uint32_t)(tok * (int)a.q.st + qc) * ES;
+  const uint32_t v_off = (uint32_t)(4 * cg * (int)a.v.st + vc) * ES, g_off = (uint32_t)(col * (int)a.g.st) * 4, b_off = (uint32_t)(col * (int)a.beta.st) * 4;
   Quad<IO, VEC> nk[SB] = {}, nq[TRANS ? 1 : SB] = {};
   IO nv[SB][4] = {};
   float ng = 0.f, nb = 0.f;
-  auto fetch = [&](int c) {
+  auto fetch = [&](int c) {                               // chunks behind the last one: the last one again, masked when used
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
-      int t = 16 * (c + i) + tok;
-      t = t < last ? t : last;
-      read4(nk[i], kp + t * a.k.st, nqk);
-      if (!TRANS) read4(nq[i], qp + t * a.q.st, nqk);
-    }
-    int tg = 16 * (c + (SB < NW ? w % SB : w)) + col;
-    tg = tg < last ? tg : last;
-    ng = gp[tg * a.g.st];
-    nb = bp[tg * a.beta.st];
-    if (!unit) {
+      const int ci = c + i < s.chunks ? c + i : s.chunks - 1, left = s.T - 1 - 16 * ci;
+      const IO* kb = kp + (int64_t)(16 * ci) * a.k.st;
+      const IO* qb = qp + (int64_t)(16 * ci) * a.q.st;
+      const IO* vb = vp + (int64_t)(16 * ci) * a.v.st;
+      if (left >= 15) {
+        read4(nk[i], by(kb, k_off), nqk);
+        if (!TRANS) read4(nq[i], by(qb, q_off), nqk);
+        if (!unit) {
 #pragma unroll
-      for (int i = 0; i < SB; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          int t = 16 * (c + i) + 4 * cg + r;
-          t = t < last ? t : last;
-          nv[i][r] = vp[t * a.v.st];
+          for (int r = 0; r < 4; ++r) nv[i][r] = *by(vb + r * a.v.st, v_off);
         }
+      } else {                                            // rows behind the tensor: its last one
+        const int t = tok < left ? tok : left;
+        read4(nk[i], by(kb, (uint32_t)(t * (int)a.k.st + qc) * ES), nqk);
+        if (!TRANS) read4(nq[i], by(qb, (uint32_t)(t * (int)a.q.st + qc) * ES), nqk);
+        if (!unit) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) nv[i][r] = *by(vb, (uint32_t)((4 * cg + r < left ? 4 * cg + r : left) * (int)a.v.st + vc) * ES);
+        }
+      }
+    }
+    const int cw = c + (SB < NW ? w % SB : w), ci = cw < s.chunks ? cw : s.chunks - 1, left = s.T - 1 - 16 * ci;
+    const float* gb = gp + (int64_t)(16 * ci) * a.g.st;
+    const float* bb = bp + (int64_t)(16 * ci) * a.beta.st;
+    if (left >= 15) {
+      ng = *by(gb, g_off);
+      nb = *by(bb, b_off);
+    } else {
+      const int t = col < left ? col : left;
+      ng = *by(gb, (uint32_t)(t * (int)a.g.st) * 4);
+      nb = *by(bb, (uint32_t)(t * (int)a.beta.st) * 4);
     }
   };
   const int64_t row_v = (int64_t)s.N * s.H * V;           // one step on in o and e
-  const int64_t out0 = ((int64_t)sq.b * s.T * s.N + sq.n) * s.H * V + (int64_t)sq.h * V + 4 * cg * row_v + n;
+  const int64_t out0 = ((int64_t)sq.b * s.T * s.N + sq.n) * s.H * V + (int64_t)sq.h * V;
+  const uint32_t o_off = (uint32_t)(4 * cg * (int)row_v + n);
   if (c0 < ce) fetch(c0);
   for (int c = c0; c < ce; c += SB) {
 #pragma unroll
@@ -152,13 +169,13 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
       if (do_inv) {
         const gd_f4 bj = lds4(&L.beta[i][4 * cg]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) kk[r] = 4 * cg + r < col ? dec[r] * kk[r] * bj[r] : 0.f;
+        for (int r = 0; r < 4; ++r) kk[r] = 4 * cg + r < col ? -(dec[r] * kk[r] * bj[r]) : 0.f;
         put4(&L.am[w][col * TS + 4 * cg], kk);
         gd_wave_sync();
         float arow[16];
         row16(&L.am[w][col * TS], arow);
         gd_f4 inv = unit_row(lane);
-        solve_down<0>(arow, inv);
+        solve_down(arow, inv);
         put4(&L.inv[i][4 * lane], inv);
       }
     }
@@ -217,22 +234,22 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
         o = mma16(pm, u, o);
         if (sq.live && vin) {
           const int64_t at = out0 + (int64_t)(16 * (c + i)) * row_v;
-          const int left = s.T - 16 * (c + i) - 4 * cg;
           IO* op = reinterpret_cast<IO*>(a.o) + at;
           float* ep = a.e + at;
           if (16 * (c + i) + 16 <= s.T) {                 // a whole chunk: no lane asks
 #pragma unroll
-            for (int r = 0; r < 4; ++r) op[r * row_v] = from_f32<IO>(o[r]);
+            for (int r = 0; r < 4; ++r) *by(op + r * row_v, o_off * ES) = from_f32<IO>(o[r]);
             if (a.e) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) ep[r * row_v] = e[r];
+              for (int r = 0; r < 4; ++r) *by(ep + r * row_v, o_off * 4) = e[r];
             }
           } else {
+            const int left = s.T - 16 * (c + i) - 4 * cg;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
               if (r < left) {
-                op[r * row_v] = from_f32<IO>(o[r]);
-                if (a.e) ep[r * row_v] = e[r];
+                *by(op + r * row_v, o_off * ES) = from_f32<IO>(o[r]);
+                if (a.e) *by(ep + r * row_v, o_off * 4) = e[r];
               }
           }
         }
@@ -398,6 +415,11 @@ int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s) {
   if (s->segs < 3) { s->segs = 1; s->cps = s->chunks > 0 ? s->chunks : 1; }
   return PGT_OK;
 }
+// a lane's offset inside sixteen steps has 32 bits
+bool pgt_delta_near(const pgt_delta_dims* d, const pgt_seq_view* v, int size) {
+  const int64_t st = v->step < 0 ? -v->step : v->step;
+  return d->steps <= 1 || (st < ((int64_t)1 << 31) / (16 * size) - 128 && v->step >= 0);
+}
 gd::View pgt_delta_view(const pgt_seq_view* v) { return gd::View{v->data, v->batch, v->step, v->node, v->head}; }
 bool pgt_delta_vec(const pgt_seq_view* v, int width, int dtype) {
   const int64_t strides = v->batch | v->step | v->node | v->head;
@@ -419,6 +441,10 @@ extern "C" int pgt_gated_delta_fwd(const pgt_delta_dims* d, const pgt_seq_view* 
   PGT_REQUIRE(last, "pgt_gated_delta_fwd: null pointer");
   if (a.s.T > 0) {
     PGT_REQUIRE(q && k && v && g && beta && q->data && k->data && v->data && g->data && beta->data && o, "pgt_gated_delta_fwd: null pointer");
+    const int es = d->dtype == PGT_DT_F32 ? 4 : 2;
+    PGT_REQUIRE(pgt_delta_near(d, q, es) && pgt_delta_near(d, k, es) && pgt_delta_near(d, v, es) && pgt_delta_near(d, g, 4) && pgt_delta_near(d, beta, 4),
+                "pgt_gated_delta_fwd: a step's stride is negative or above 2^27 bytes");
+    PGT_REQUIRE(d->nodes * d->heads * d->value < ((int64_t)1 << 25) - 128, "pgt_gated_delta_fwd: more than 2^25 values a step and sample");
     a.q = pgt_delta_view(q); a.k = pgt_delta_view(k); a.v = pgt_delta_view(v); a.g = pgt_delta_view(g); a.beta = pgt_delta_view(beta);
     a.vec = pgt_delta_vec(q, a.s.K, d->dtype) && pgt_delta_vec(k, a.s.K, d->dtype) && pgt_delta_vec(v, a.s.V, d->dtype);
   } else {
