@@ -22,6 +22,22 @@ struct f16 { uint16_t u; };
 #else
 typedef float gd_f4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ gd_f4 gd_mfma(float a, float b, gd_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// bf16 products: eight contraction values a lane, packed in pairs.  (This shape only: with hipcc 7.2 a 16x16x16 MFMA right behind a
+// 16x16x32 one on the same accumulator summed wrongly on gfx950; four values are filled up with zeros instead.)
+typedef uint32_t gd_h8 __attribute__((ext_vector_type(4)));
+typedef uint32_t gd_h4 __attribute__((ext_vector_type(2)));
+typedef __bf16 gd_bf8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ gd_f4 gd_mfma32(gd_h8 a, gd_h8 b, gd_f4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gd_bf8, a), __builtin_bit_cast(gd_bf8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ gd_h8 gd_join(gd_h4 x, gd_h4 y) { return gd_h8{x.x, x.y, y.x, y.y}; }
+__device__ __forceinline__ gd_h4 gd_mk_h4(uint32_t lo, uint32_t hi) { return gd_h4{lo, hi}; }
+typedef float gd_f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 gd_bf2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t gd_pack_bf16(float x, float y) {       // v_cvt_pk_bf16_f32: round to nearest even
+  const gd_f2 v = {x, y};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, gd_bf2));
+}
 // value of lane J of the row of sixteen (DPP row_newbcast)
 template <int J> __device__ __forceinline__ float gd_bcast16(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + J, 0xf, 0xf, true));
@@ -87,12 +103,33 @@ __device__ __forceinline__ gd_f4 lds4(const float* p) {
   r[0] = t.x; r[1] = t.y; r[2] = t.z; r[3] = t.w;
   return r;
 }
+__device__ __forceinline__ gd_h4 lds_h4(const uint16_t* p) { const int2 t = *reinterpret_cast<const int2*>(p); return gd_mk_h4((uint32_t)t.x, (uint32_t)t.y); }
 __device__ __forceinline__ void put4(float* p, gd_f4 x) { *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]); }
 // c += A B over sixteen contraction steps, k = 4 (l / 16) + r
 __device__ __forceinline__ gd_f4 mma16(gd_f4 a, gd_f4 b, gd_f4 c) {
 #pragma unroll
   for (int r = 0; r < 4; ++r) c = gd_mfma(a[r], b[r], c);
   return c;
+}
+// Four fp32 values as three bf16 pieces each (24 bits in all): x = p1 + p2 + p3 up to 2^-24 of x.  A product with an operand that IS
+// bf16 is then three MFMAs on the bf16 pipe, sixteen times the fp32 pipe's rate, and as exact as fp32.
+struct Split { gd_h4 p1, p2, p3; };
+__device__ __forceinline__ gd_h8 half_of(gd_h4 x) { return gd_join(x, gd_mk_h4(0u, 0u)); }
+__device__ __forceinline__ Split split4(gd_f4 x) {
+  uint32_t a[3], b[3];
+  float r0 = x[0], r1 = x[1], r2 = x[2], r3 = x[3];
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    a[i] = gd_pack_bf16(r0, r1);
+    b[i] = gd_pack_bf16(r2, r3);
+    if (i < 2) {
+      r0 -= gd_as_float(a[i] << 16); r1 -= gd_as_float(a[i] & 0xffff0000u);
+      r2 -= gd_as_float(b[i] << 16); r3 -= gd_as_float(b[i] & 0xffff0000u);
+    }
+  }
+  Split s;
+  s.p1 = gd_mk_h4(a[0], b[0]); s.p2 = gd_mk_h4(a[1], b[1]); s.p3 = gd_mk_h4(a[2], b[2]);
+  return s;
 }
 __device__ __forceinline__ float sum16(float x) {       // the sum over the row of sixteen lanes, in every one of them
   x += gd_ror16<8>(x);
@@ -248,6 +285,17 @@ inline int fresh(int x) { return x; }
 #else
 __device__ __forceinline__ int fresh(int x) { asm volatile("" : "+v"(x)); return x; }
 #endif
+// a bf16 quad as it is, masked
+__device__ __forceinline__ int2 raw(const Quad<bf16, true>& q, int n) { int2 r = q.x; if (n <= 0) r.x = r.y = 0; return r; }
+__device__ __forceinline__ int2 raw(const Quad<bf16, false>& q, int n) {
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = n > i ? q.x[i].u : 0u;
+  int2 r;
+  r.x = (int)(v[0] | (v[1] << 16));
+  r.y = (int)(v[2] | (v[3] << 16));
+  return r;
+}
 // Waits for a load here.  A load that is used behind stores whose number the compiler cannot know would wait for the stores as well.
 #ifdef PGT_EMU
 template <class T> inline void arrive(T&) {}

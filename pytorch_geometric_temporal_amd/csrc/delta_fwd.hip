@@ -1,5 +1,7 @@
 // Gated delta rule, whole sequences, forward (delta_common.h has the formulas).
 #include "delta_common.h"
+
+#include <type_traits>
 #include <stdlib.h>
 
 using namespace gd;
@@ -30,8 +32,11 @@ template <class IO, int D, bool TRANS, bool FULL, bool VEC>
 __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void delta_fwd_kernel(FwdArgs a) {
   using TM = Team<D>;
   constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, SB = TM::SB, TB = 16 * SB, NT = D / 16;
+  constexpr bool HALF = std::is_same_v<IO, bf16>;          // keys and queries stay bf16 in LDS, products with them run on the bf16 pipe
+  constexpr int LH = D + 8;                                // row stride of the bf16 tiles, in values
   struct Lds {
-    float k[TB * LD], q[TRANS ? 4 : TB * LD];
+    float k[HALF ? 4 : TB * LD], q[HALF || TRANS ? 4 : TB * LD];
+    uint16_t kb[HALF ? TB * LH : 8], qb[HALF && !TRANS ? TB * LH : 8];
     float inv[SB][256], p[TRANS ? 1 : SB][256];           // A operands, four values a lane
     float am[NW][TILE];
     float hi[NW][16], lo[NW][16], enter[SB][16], leave[SB][16], beta[SB][16], whole[SB];
@@ -124,6 +129,11 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
       const int have = 16 * (c + i) + tok < sq.len ? nqk : 0;
+      if constexpr (HALF) {
+        *reinterpret_cast<int2*>(&L.kb[(16 * i + tok) * LH + qd]) = raw(nk[i], have);
+        if (!TRANS) *reinterpret_cast<int2*>(&L.qb[(16 * i + tok) * LH + qd]) = raw(nq[i], have);
+        continue;
+      }
       put4(&L.k[(16 * i + tok) * LD + qd], unpack(nk[i], have));
       if (!TRANS) {
         gd_f4 x = unpack(nq[i], have);
@@ -150,6 +160,23 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
         if (do_inv) { L.enter[i][lane] = d.enter; L.leave[i][lane] = d.leave; L.beta[i][lane] = b; if (lane == 0) L.whole[i] = d.whole; }
       }
       gd_f4 kk = zero4(), kq = zero4();                   // row j = 4 cg + r, column i = col: the A operand's layout of the transposed tile
+      if constexpr (HALF) {
+        const uint16_t* kr = &L.kb[(16 * i + col) * LH + 4 * cg];
+        const uint16_t* qr = &L.qb[TRANS ? 0 : (16 * i + col) * LH + 4 * cg];
+#pragma unroll
+        for (int t = 0; t + 1 < NT; t += 2) {
+          const gd_h8 x = gd_join(lds_h4(kr + 16 * t), lds_h4(kr + 16 * t + 16));
+          if (do_inv) kk = gd_mfma32(x, x, kk);
+          if (do_p) kq = gd_mfma32(x, gd_join(lds_h4(qr + 16 * t), lds_h4(qr + 16 * t + 16)), kq);
+        }
+        if (NT % 2) {
+          const gd_h8 x = half_of(lds_h4(kr + 16 * (NT - 1)));
+          if (do_inv) kk = gd_mfma32(x, x, kk);
+          if (do_p) kq = gd_mfma32(x, half_of(lds_h4(qr + 16 * (NT - 1))), kq);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) kq[r] *= s.scale;
+      } else
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         const gd_f4 x = lds4(&L.k[(16 * i + col) * LD + 16 * t + 4 * cg]);
@@ -205,6 +232,33 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
 #pragma unroll
       for (int j = 0; j + 1 < SB; ++j) v[j] = v[j + 1];
       if (!zero) {
+        if constexpr (HALF) {
+          const uint16_t* kr = &L.kb[(16 * i + col) * LH + 4 * cg];
+          const uint16_t* qr = &L.qb[TRANS ? 0 : (16 * i + col) * LH + 4 * cg];
+#pragma unroll
+          for (int t = 0; t + 1 < NT; t += 2) {
+            if (t % 4 == 0) PGT_SCHED_FENCE();
+            const Split a0 = split4(S[t]), a1 = split4(S[t + 1]);
+            const gd_h8 p1 = gd_join(a0.p1, a1.p1), p2 = gd_join(a0.p2, a1.p2), p3 = gd_join(a0.p3, a1.p3);
+            const gd_h8 x = gd_join(lds_h4(kr + 16 * t), lds_h4(kr + 16 * t + 16));
+            ks = gd_mfma32(x, p3, gd_mfma32(x, p2, gd_mfma32(x, p1, ks)));
+            if (!TRANS) {
+              const gd_h8 z = gd_join(lds_h4(qr + 16 * t), lds_h4(qr + 16 * t + 16));
+              o = gd_mfma32(z, p3, gd_mfma32(z, p2, gd_mfma32(z, p1, o)));
+            }
+          }
+          if (NT % 2) {
+            const Split a0 = split4(S[NT - 1]);
+            const gd_h4 x = lds_h4(kr + 16 * (NT - 1));
+            ks = gd_mfma32(half_of(x), half_of(a0.p3), gd_mfma32(gd_join(x, x), gd_join(a0.p1, a0.p2), ks));
+            if (!TRANS) {
+              const gd_h4 z = lds_h4(qr + 16 * (NT - 1));
+              o = gd_mfma32(half_of(z), half_of(a0.p3), gd_mfma32(gd_join(z, z), gd_join(a0.p1, a0.p2), o));
+            }
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] *= s.scale;
+        } else
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           if (t % 4 == 0) PGT_SCHED_FENCE();
@@ -221,6 +275,20 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
       gd_f4 u, ul;
 #pragma unroll
       for (int r = 0; r < 4; ++r) { u[r] = beta[r] * e[r]; ul[r] = leave[r] * u[r]; }
+      if constexpr (HALF) {
+        const Split us = split4(ul);
+        const gd_h8 u12 = gd_join(us.p1, us.p2), u3 = half_of(us.p3);
+        const uint16_t* kc = &L.kb[(16 * i + 4 * cg) * LH + col];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          if (t % 4 == 0) PGT_SCHED_FENCE();
+          const gd_h4 kt = gd_mk_h4((uint32_t)kc[16 * t] | ((uint32_t)kc[LH + 16 * t] << 16),
+                                    (uint32_t)kc[2 * LH + 16 * t] | ((uint32_t)kc[3 * LH + 16 * t] << 16));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) S[t][r] *= whole;
+          S[t] = gd_mfma32(half_of(kt), u3, gd_mfma32(gd_join(kt, kt), u12, S[t]));
+        }
+      } else
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (t % 4 == 0) PGT_SCHED_FENCE();
@@ -280,8 +348,9 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
 // x [P, segs - 1, K, V] holds the second summand and takes the sum (its entry 0 is complete already).  UP (the adjoint): from the last
 // entry down with the transposed transitions.  A workgroup owns sixteen columns of a sequence's state, a wavefront sixteen rows; the
 // next two transitions are on their way while one is multiplied: what remains of a step is its K / 4 dependent MFMAs and one barrier.
-template <int D, bool UP, bool VEC>
-__global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K, int V) {
+template <int D, bool UP, bool VEC, bool FULL>
+__global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K_, int V_) {
+  const int K = FULL ? D : K_, V = FULL ? D : V_;       // FULL: every lane stores, and the compiler knows how much is in flight
   constexpr int LD = D + 4, NT = D / 16;
   __shared__ __attribute__((aligned(16))) float st[2][16 * LD];     // [column][row], two buffers
   const int w = (int)threadIdx.x / 64, lane = (int)threadIdx.x & 63, col = lane & 15, cg = lane >> 4;
@@ -326,7 +395,7 @@ __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* 
     fetch(j + 2 < entries ? j + 2 : entries - 1, m, add);  // (always: with a branch here every step would wait for all loads)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
-      if (row0 + r < K && n < V) xp[((int64_t)to * K + r) * V] = s[r];
+      if (FULL || (row0 + r < K && n < V)) xp[((int64_t)to * K + r) * V] = s[r];
   };
   fetch(1, m0, add0);
   fetch(entries > 2 ? 2 : 1, m1, add1);
@@ -351,8 +420,9 @@ template <class IO, int D, bool TRANS, bool FULL, bool VEC> void go(const FwdArg
 }
 template <int D, bool UP> void join(const float* trans, float* x, int64_t P, int segs, int K, int V, pgt_stream_t stream) {
   const dim3 grid((unsigned)P, (unsigned)((V + 15) / 16)), block(64 * (D / 16));
-  if (!UP && K % 4 == 0 && pgt_aligned(trans, 16)) PGT_LAUNCH((delta_join_kernel<D, UP, !UP>), grid, block, stream, trans, x, segs, K, V);
-  else PGT_LAUNCH((delta_join_kernel<D, UP, false>), grid, block, stream, trans, x, segs, K, V);
+  if (K == D && V == D && pgt_aligned(trans, 16)) PGT_LAUNCH((delta_join_kernel<D, UP, !UP, true>), grid, block, stream, trans, x, segs, K, V);
+  else if (!UP && K % 4 == 0 && pgt_aligned(trans, 16)) PGT_LAUNCH((delta_join_kernel<D, UP, !UP, false>), grid, block, stream, trans, x, segs, K, V);
+  else PGT_LAUNCH((delta_join_kernel<D, UP, false, false>), grid, block, stream, trans, x, segs, K, V);
 }
 template <class IO, int D> void all(const FwdArgs& a, pgt_stream_t stream) {
   const bool full = a.vec && a.s.K == D && a.s.V == D;

@@ -25,6 +25,35 @@ static inline gd_f4 gd_mfma(float a, float b, gd_f4 c) {
   pgt_emu::wave_barrier();
   return c;
 }
+// v_mfma_f32_16x16x32_bf16: lane l holds eight consecutive contraction values of row l % 16, group l / 16
+struct gd_h8 { uint32_t v[4]; };
+struct gd_h4 { uint32_t v[2]; };
+static uint32_t gd_emu_a[16][64][4], gd_emu_b[16][64][4];
+static inline gd_f4 gd_emu_mfma_h(const uint32_t* a, const uint32_t* b, gd_f4 c) {
+  pgt_emu::State& st = pgt_emu::S();
+  const unsigned w = st.cur / 64, lane = st.cur % 64;
+  for (int q = 0; q < 4; ++q) { gd_emu_a[w][lane][q] = a[q]; gd_emu_b[w][lane][q] = b[q]; }
+  pgt_emu::wave_barrier();
+  const unsigned col = lane & 15;
+  for (int r = 0; r < 4; ++r) {
+    const unsigned row = 4 * (lane >> 4) + r;
+    float acc = c[r];
+    for (int g = 0; g < 4; ++g)
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t wa = gd_emu_a[w][row + 16 * g][q >> 1], wb = gd_emu_b[w][col + 16 * g][q >> 1];
+        float x, y;
+        const uint32_t ba = (q & 1) ? (wa & 0xffff0000u) : (wa << 16), bb = (q & 1) ? (wb & 0xffff0000u) : (wb << 16);
+        memcpy(&x, &ba, 4); memcpy(&y, &bb, 4);
+        acc = fmaf(x, y, acc);
+      }
+    c[r] = acc;
+  }
+  pgt_emu::wave_barrier();
+  return c;
+}
+static inline gd_f4 gd_mfma32(gd_h8 a, gd_h8 b, gd_f4 c) { return gd_emu_mfma_h(a.v, b.v, c); }
+static inline gd_h8 gd_join(gd_h4 x, gd_h4 y) { gd_h8 r; r.v[0] = x.v[0]; r.v[1] = x.v[1]; r.v[2] = y.v[0]; r.v[3] = y.v[1]; return r; }
+static inline gd_h4 gd_mk_h4(uint32_t lo, uint32_t hi) { gd_h4 r; r.v[0] = lo; r.v[1] = hi; return r; }
 template <int J> static inline float gd_bcast16(float x) { return __shfl(x, (__lane_id() & 48) | J); }
 template <int N> static inline float gd_ror16(float x) { return __shfl(x, (__lane_id() & 48) | ((__lane_id() - N) & 15)); }
 template <int N> static inline double gd_shr16(double x) {          // lane i takes lane i - N of its row, 0 where there is none
@@ -44,6 +73,7 @@ static inline uint16_t gd_to_bf16(float x) {
   if ((u & 0x7fffffffu) > 0x7f800000u) return (uint16_t)((u >> 16) | 0x40u);
   return (uint16_t)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
 }
+static inline uint32_t gd_pack_bf16(float x, float y) { return (uint32_t)gd_to_bf16(x) | ((uint32_t)gd_to_bf16(y) << 16); }
 static inline float gd_from_f16(uint16_t h) {
   const uint32_t s = (uint32_t)(h & 0x8000u) << 16, e = (h >> 10) & 31u, m = h & 1023u;
   if (e == 31) return gd_as_float(s | 0x7f800000u | (m << 13));
