@@ -101,25 +101,25 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
   Quad<float, VEC> ne = {};
   float ng = 0.f, nb = 0.f;
   auto fetch = [&](int c) {
-    const int64_t t0 = 16 * c;
+    const int t0 = 16 * c;
     const int left = s.T - 1 - 16 * c;
-    const IO* kb = kp + t0 * a.k.st;
-    const IO* qb = qp + t0 * a.q.st;
-    const float* gb = gp + t0 * a.g.st;
-    const float* bb = bp + t0 * a.beta.st;
+    const IO* kb = kp + mul32(t0, a.k.st);
+    const IO* qb = qp + mul32(t0, a.q.st);
+    const float* gb = gp + mul32(t0, a.g.st);
+    const float* bb = bp + mul32(t0, a.beta.st);
     if (left >= 15) {
       read4(nk, by(kb, k_off), nqk);
       read4(nq, by(qb, q_off), nqk);
-      read4(no, by(op + t0 * row_v, v_off * ES), nvv);
-      if (!STATE) read4(ne, by(ep + t0 * row_v, v_off * 4), nvv);
+      read4(no, by(op + mul32(t0, row_v), v_off * ES), nvv);
+      if (!STATE) read4(ne, by(ep + mul32(t0, row_v), v_off * 4), nvv);
       ng = *by(gb, g_off);
       nb = *by(bb, b_off);
     } else {                                              // rows behind the tensor: its last one, masked when used
       const int t = tok < left ? tok : left, tg = col < left ? col : left;
       read4(nk, by(kb, (uint32_t)(t * (int)a.k.st + qc) * ES), nqk);
       read4(nq, by(qb, (uint32_t)(t * (int)a.q.st + qc) * ES), nqk);
-      read4(no, by(op + t0 * row_v, (uint32_t)(t * (int)row_v + vc) * ES), nvv);
-      if (!STATE) read4(ne, by(ep + t0 * row_v, (uint32_t)(t * (int)row_v + vc) * 4), nvv);
+      read4(no, by(op + mul32(t0, row_v), (uint32_t)(t * (int)row_v + vc) * ES), nvv);
+      if (!STATE) read4(ne, by(ep + mul32(t0, row_v), (uint32_t)(t * (int)row_v + vc) * 4), nvv);
       ng = *by(gb, (uint32_t)(tg * (int)a.g.st) * 4);
       nb = *by(bb, (uint32_t)(tg * (int)a.beta.st) * 4);
     }
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
       const int l = 4 * cg + r;                           // column col adds its rows >= l where col < l; step col its z where col >= l, its w where not
       dg[r] = sum16(col < l ? suf[r] + above + wj : z) + dot * whole;
     }
-    const int64_t at = seq_h + (int64_t)(16 * c) * row_h;
+    const int64_t at = seq_h + mul32(16 * c, row_h);
     if (sq.live && lane < 16 && 16 * c + lane < s.T) a.dbeta[at + lane * row_h] = 16 * c + lane < sq.len ? dbv : 0.f;
     if (sq.live && col < 4) {
       const int l = 4 * cg + col;
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
           for (int r = 0; r < 4; ++r) L.red[w][0][4 * cg + r] = db[r];
         }
         if (sq.live && vin) {
-          IO* to = reinterpret_cast<IO*>(a.dv) + (seq_h + (int64_t)(16 * c) * row_h) * V;
+          IO* to = reinterpret_cast<IO*>(a.dv) + seq_h * V + mul32(16 * c, row_v);
           const uint32_t off = (uint32_t)(4 * cg * (int)row_v + n) * ES;
           if (16 * c + 16 <= s.T) {
 #pragma unroll
@@ -408,20 +408,17 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
         }
         const gd_f4 bt = take(4);
         const gd_f4 m1t = lds4(&L.m1[col * TS + 4 * cg]);
-        // entry (i = col, j = 4 cg + r) of D beta, where `bt` has (i = 4 cg + r, j = col): with lane 16 (col / 4) + 4 cg + r as value col % 4
-        auto mirror = [&](int r) {
-          const int from_lane = 16 * (col >> 2) + 4 * cg + r;
-          if (NW > 1) return L.lane4[NW > 1 ? 4 : 0][NW > 1 ? 4 * from_lane + (col & 3) : 0];
-          const float v0 = __shfl(bt[0], from_lane), v1 = __shfl(bt[1], from_lane), v2 = __shfl(bt[2], from_lane), v3 = __shfl(bt[3], from_lane);
-          return (col & 3) == 0 ? v0 : (col & 3) == 1 ? v1 : (col & 3) == 2 ? v2 : v3;
-        };
+        // D_ij beta_j for (i = col, j = 4 cg + r), where `bt` has (i = 4 cg + r, j = col): computed again, cheaper than turned in LDS
+        const gd_f4 hj = lds4(&L.hi[0][4 * cg]), lj = lds4(&L.lo[0][4 * cg]);
+        const float hc = L.hi[0][col], lc = L.lo[0][col];
         gd_f4 kc, qc, m1;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           kc[r] = L.k[(4 * cg + r) * LD + n];
           qc[r] = L.q[(4 * cg + r) * LD + n];
           m1[r] = L.m1[(4 * cg + r) * TS + col];
-          m2[r] = -(m2[r] * mirror(r)) - m2t[r] * bt[r];
+          const float turned = 4 * cg + r < col ? gd_exp2((hc - hj[r]) + (lc - lj[r])) * beta[r] : 0.f;
+          m2[r] = -(m2[r] * turned) - m2t[r] * bt[r];
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -441,7 +438,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
         if (sq.live && kin) {
           const int left = s.T - 16 * c - 4 * cg;
           const int64_t row_k = (s.rep > 1 ? row_h : (int64_t)s.N * (s.H / s.rep)) * K;
-          const int64_t at = (s.rep > 1 ? seq_h : ((int64_t)sq.b * s.T * s.N + sq.n) * (s.H / s.rep) + kh) * K + (int64_t)(16 * c) * row_k;
+          const int64_t at = (s.rep > 1 ? seq_h : ((int64_t)sq.b * s.T * s.N + sq.n) * (s.H / s.rep) + kh) * K + mul32(16 * c, row_k);
           const uint32_t off = (uint32_t)(4 * cg * (int)row_k + n);
           auto put = [&](auto* dq, auto* dk, int r) {
             using T = std::remove_pointer_t<decltype(dq)>;
@@ -498,7 +495,9 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
 
 // y[row, kh, :] = sum over the key head's value heads of x[row, kh rep + i, :], in head order
 template <class IO>
-__global__ __launch_bounds__(256) void delta_heads_kernel(const float* x, IO* y, int64_t n, int rep, int K) {
+__global__ __launch_bounds__(256) void delta_heads_kernel(const float* x, IO* dq, IO* dk, int64_t n, int rep, int K) {
+  IO* y = blockIdx.y == 0 ? dq : dk;
+  x += blockIdx.y * n * rep;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   const int64_t head = i / K;
@@ -540,9 +539,8 @@ template <class IO> int by_width(const BwdArgs& a0, void* dq, void* dk, const fl
   if (e || a.s.rep == 1) return e;
   const int64_t n = (a.s.P / a.s.rep) * a.s.T * a.s.K;
   if (n == 0) return PGT_OK;
-  const dim3 grid((unsigned)pgt_cdiv(n, 256));
-  PGT_LAUNCH((delta_heads_kernel<IO>), grid, dim3(256), stream, (const float*)a.dq, (IO*)dq, n, a.s.rep, a.s.K);
-  PGT_LAUNCH((delta_heads_kernel<IO>), grid, dim3(256), stream, (const float*)a.dk, (IO*)dk, n, a.s.rep, a.s.K);
+  const dim3 grid((unsigned)pgt_cdiv(n, 256), 2);
+  PGT_LAUNCH((delta_heads_kernel<IO>), grid, dim3(256), stream, (const float*)a.dq, (IO*)dq, (IO*)dk, n, a.s.rep, a.s.K);
   return pgt_check_launch("pgt_gated_delta_bwd");
 }
 
@@ -560,7 +558,7 @@ extern "C" int pgt_gated_delta_bwd(const pgt_delta_dims* d, const pgt_seq_view* 
                 "pgt_gated_delta_bwd: null pointer");
     const int es = d->dtype == PGT_DT_F32 ? 4 : 2;
     PGT_REQUIRE(pgt_delta_near(d, q, es) && pgt_delta_near(d, k, es) && pgt_delta_near(d, g, 4) && pgt_delta_near(d, beta, 4),
-                "pgt_gated_delta_bwd: a step's stride is negative or above 2^27 bytes");
+                "pgt_gated_delta_bwd: a stride is negative, a step's above 2^27 bytes or a node's or head's above 2^31 values");
     PGT_REQUIRE(d->nodes * d->heads * d->value < ((int64_t)1 << 25) - 128 && d->nodes * d->heads * d->key < ((int64_t)1 << 25) - 128,
                 "pgt_gated_delta_bwd: more than 2^25 values a step and sample");
     PGT_REQUIRE(a.s.chunks == 1 || states, "pgt_gated_delta_bwd: %d chunks need the forward pass's states", a.s.chunks);

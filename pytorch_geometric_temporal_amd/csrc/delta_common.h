@@ -310,8 +310,11 @@ template <class IO> __device__ __forceinline__ void arrive(Quad<IO, false>& q) {
 // p (the same in every lane) and a lane's own offset in bytes: one scalar base and one register, no 64-bit sum a lane
 template <class T> __device__ __forceinline__ const T* by(const T* p, uint32_t bytes) { return reinterpret_cast<const T*>(reinterpret_cast<const char*>(p) + bytes); }
 template <class T> __device__ __forceinline__ T* by(T* p, uint32_t bytes) { return reinterpret_cast<T*>(reinterpret_cast<char*>(p) + bytes); }
+// 32 x 32 -> 64 bits: two scalar instructions where a 64-bit product takes six
+__device__ __forceinline__ int64_t mul32(int a, int64_t b) { return (int64_t)((uint64_t)(uint32_t)a * (uint32_t)b); }
+// (strides but the sample's are below 2^31: the host sees to it)
 template <class T> __device__ __forceinline__ const T* at(const View& v, const Seq& q, int h) {
-  return reinterpret_cast<const T*>(v.p) + (int64_t)q.b * v.sb + (int64_t)q.n * v.sn + (int64_t)h * v.sh;
+  return reinterpret_cast<const T*>(v.p) + (int64_t)q.b * v.sb + mul32(q.n, v.sn) + mul32(h, v.sh);
 }
 // chunks that any of the workgroup's sequences reaches (the same in every thread)
 template <int TEAMS> __device__ __forceinline__ int chunks_of_block(const Shape& s, int64_t first) {

@@ -89,9 +89,9 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
 #pragma unroll
     for (int i = 0; i < SB; ++i) {
       const int ci = c + i < s.chunks ? c + i : s.chunks - 1, left = s.T - 1 - 16 * ci;
-      const IO* kb = kp + (int64_t)(16 * ci) * a.k.st;
-      const IO* qb = qp + (int64_t)(16 * ci) * a.q.st;
-      const IO* vb = vp + (int64_t)(16 * ci) * a.v.st;
+      const IO* kb = kp + mul32(16 * ci, a.k.st);
+      const IO* qb = qp + mul32(16 * ci, a.q.st);
+      const IO* vb = vp + mul32(16 * ci, a.v.st);
       if (left >= 15) {
         read4(nk[i], by(kb, k_off), nqk);
         if (!TRANS) read4(nq[i], by(qb, q_off), nqk);
@@ -110,8 +110,8 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
       }
     }
     const int cw = c + (SB < NW ? w % SB : w), ci = cw < s.chunks ? cw : s.chunks - 1, left = s.T - 1 - 16 * ci;
-    const float* gb = gp + (int64_t)(16 * ci) * a.g.st;
-    const float* bb = bp + (int64_t)(16 * ci) * a.beta.st;
+    const float* gb = gp + mul32(16 * ci, a.g.st);
+    const float* bb = bp + mul32(16 * ci, a.beta.st);
     if (left >= 15) {
       ng = *by(gb, g_off);
       nb = *by(bb, b_off);
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
       if (!TRANS) {
         o = mma16(pm, u, o);
         if (sq.live && vin) {
-          const int64_t at = out0 + (int64_t)(16 * (c + i)) * row_v;
+          const int64_t at = out0 + mul32(16 * (c + i), row_v);
           IO* op = reinterpret_cast<IO*>(a.o) + at;
           float* ep = a.e + at;
           if (16 * (c + i) + 16 <= s.T) {                 // a whole chunk: no lane asks
@@ -488,7 +488,8 @@ int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s) {
 // a lane's offset inside sixteen steps has 32 bits
 bool pgt_delta_near(const pgt_delta_dims* d, const pgt_seq_view* v, int size) {
   const int64_t st = v->step < 0 ? -v->step : v->step;
-  return d->steps <= 1 || (st < ((int64_t)1 << 31) / (16 * size) - 128 && v->step >= 0);
+  const int64_t top = (int64_t)1 << 31;
+  return v->node >= 0 && v->node < top && v->head >= 0 && v->head < top && (d->steps <= 1 || (st < top / (16 * size) - 128 && v->step >= 0));
 }
 gd::View pgt_delta_view(const pgt_seq_view* v) { return gd::View{v->data, v->batch, v->step, v->node, v->head}; }
 bool pgt_delta_vec(const pgt_seq_view* v, int width, int dtype) {
@@ -513,7 +514,7 @@ extern "C" int pgt_gated_delta_fwd(const pgt_delta_dims* d, const pgt_seq_view* 
     PGT_REQUIRE(q && k && v && g && beta && q->data && k->data && v->data && g->data && beta->data && o, "pgt_gated_delta_fwd: null pointer");
     const int es = d->dtype == PGT_DT_F32 ? 4 : 2;
     PGT_REQUIRE(pgt_delta_near(d, q, es) && pgt_delta_near(d, k, es) && pgt_delta_near(d, v, es) && pgt_delta_near(d, g, 4) && pgt_delta_near(d, beta, 4),
-                "pgt_gated_delta_fwd: a step's stride is negative or above 2^27 bytes");
+                "pgt_gated_delta_fwd: a stride is negative, a step's above 2^27 bytes or a node's or head's above 2^31 values");
     PGT_REQUIRE(d->nodes * d->heads * d->value < ((int64_t)1 << 25) - 128, "pgt_gated_delta_fwd: more than 2^25 values a step and sample");
     a.q = pgt_delta_view(q); a.k = pgt_delta_view(k); a.v = pgt_delta_view(v); a.g = pgt_delta_view(g); a.beta = pgt_delta_view(beta);
     a.vec = pgt_delta_vec(q, a.s.K, d->dtype) && pgt_delta_vec(k, a.s.K, d->dtype) && pgt_delta_vec(v, a.s.V, d->dtype);

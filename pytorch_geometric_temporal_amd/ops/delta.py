@@ -33,6 +33,12 @@ def _last_axis_contiguous(t):
     return t if t.stride(-1) == 1 or t.size(-1) <= 1 else t.contiguous()
 
 
+def _in_reach(t):
+    """The kernels take strides of up to 2^25 values from step to step and 2^31 from node to node and head to head."""
+    st = t.stride()
+    return t if st[1] < 1 << 25 and st[2] < 1 << 31 and st[3] < 1 << 31 else t.contiguous()
+
+
 def on_device(t):
     """The tensor's device as the current one, where it is not (a launch goes to a stream of the current device)."""
     return contextlib.nullcontext() if not t.is_cuda or t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
@@ -87,15 +93,22 @@ def _forward(q, k, v, g, beta, start, lengths, scale, keep):
         raise _lib.PgtError(f"gated_delta_rule: {lib.last_error()}")
     o = torch.empty(B, T, N, H, V, dtype=v.dtype, device=dev)
     last = torch.empty(B, N, H, K, V, dtype=F32, device=dev)
-    e = torch.empty(B, T, N, H, V, dtype=F32, device=dev) if keep else None
-    states = torch.empty(P, (T + 15) // 16 - 1, K, V, dtype=F32, device=dev) if keep and T > 16 else None
-    seg_start = torch.empty(P, segs - 1, K, V, dtype=F32, device=dev) if segs > 1 else None
-    seg_trans = torch.empty(P, segs - 2, K, K, dtype=F32, device=dev) if segs > 1 else None
+    # one buffer: the segments' transitions, the misses e and the chunks' states (kept for the adjoint), the segments' start states
+    n_trans, n_start = (P * (segs - 2) * K * K, P * (segs - 1) * K * V) if segs > 1 else (0, 0)
+    n_e, n_states = (P * T * V, P * max((T + 15) // 16 - 1, 0) * K * V) if keep else (0, 0)
+    at_e = -(-n_trans // 4) * 4                            # (parts start at multiples of 16 bytes)
+    at_states = at_e + -(-n_e // 4) * 4
+    at_start = at_states + -(-n_states // 4) * 4
+    buf, base = None, 0
+    if at_start + n_start:
+        buf = torch.empty(at_start + n_start, dtype=F32, device=dev)
+        base = buf.data_ptr()
     arr, views = _views(q, k, v, g, beta)
     _timed("gated_delta", 7.0 * P * T * K * V if KERNEL_TIMER else 0, lambda: lib.call(
-        "pgt_gated_delta_fwd", dims, *views, ptr(start), ptr(o), ptr(last), ptr(e), ptr(states), ptr(seg_start), ptr(seg_trans),
+        "pgt_gated_delta_fwd", dims, *views, ptr(start), ptr(o), ptr(last), base + 4 * at_e if n_e else None,
+        base + 4 * at_states if n_states else None, base + 4 * at_start if segs > 1 else None, base if segs > 1 else None,
         stream_of(lib, v)))
-    return o, last, (e, states, seg_trans)
+    return o, last, buf, (segs, at_e, at_states)
 
 
 class GatedDeltaFunction(torch.autograd.Function):
@@ -104,8 +117,8 @@ class GatedDeltaFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, start, lengths, scale):
-        o, last, kept = _forward(q, k, v, g, beta, start, lengths, scale, True)
-        ctx.save_for_backward(q, k, g, beta, start, lengths, *kept)
+        o, last, buf, ctx.parts = _forward(q, k, v, g, beta, start, lengths, scale, True)
+        ctx.save_for_backward(q, k, g, beta, start, lengths, buf)
         ctx.like, ctx.scale = (v.size(3), v.size(4)), scale
         ctx.set_materialize_grads(False)
         return o, last
@@ -114,10 +127,10 @@ class GatedDeltaFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_last):
         lib = _lib.get_lib()
-        q, k, g, beta, start, lengths, e, states, seg_trans = ctx.saved_tensors
+        q, k, g, beta, start, lengths, buf = ctx.saved_tensors
         B, T, N, Hk, K = q.shape
         (H, V), scale, dtype, dev = ctx.like, ctx.scale, q.dtype, q.device
-        P, segs = B * N * H, 1 if seg_trans is None else seg_trans.size(1) + 2
+        P, (segs, at_e, at_states) = B * N * H, ctx.parts
         if d_o is None and d_last is None:
             return (None,) * 8
         d_o = torch.zeros(B, T, N, H, V, dtype=dtype, device=dev) if d_o is None else d_o.contiguous()
@@ -125,16 +138,18 @@ class GatedDeltaFunction(torch.autograd.Function):
         dq = torch.empty(B, T, N, Hk, K, dtype=dtype, device=dev)
         dk = torch.empty_like(dq)
         dv = torch.empty(B, T, N, H, V, dtype=dtype, device=dev)
-        dg = torch.empty(B, T, N, H, dtype=F32, device=dev)
-        dbeta = torch.empty_like(dg)
+        dgb = torch.empty(2, B, T, N, H, dtype=F32, device=dev)
+        dg, dbeta = dgb[0], dgb[1]
         d_start = torch.empty(B, N, H, K, V, dtype=F32, device=dev) if start is not None and ctx.needs_input_grad[5] else None
-        head_ws = torch.empty(2, P * T * K, dtype=F32, device=dev) if H > Hk else None
-        seg_end = torch.empty(P, segs - 1, K, V, dtype=F32, device=dev) if segs > 1 else None
+        n_heads, n_end = 2 * P * T * K if H > Hk else 0, P * (segs - 1) * K * V
+        ws = torch.empty(n_end + n_heads, dtype=F32, device=dev) if n_end + n_heads else None
+        base, kept = ptr(ws) or 0, ptr(buf) or 0
         dims = DeltaDimsStruct(B, T, N, Hk, H, K, V, DTYPES[dtype], scale, ptr(lengths))
         arr, (qv, kv, _, gv, bv) = _views(q, k, d_o, g, beta)
         _timed("gated_delta_bwd", 14.0 * P * T * K * V if KERNEL_TIMER else 0, lambda: lib.call(
-            "pgt_gated_delta_bwd", dims, qv, kv, gv, bv, ptr(start), ptr(e), ptr(states), ptr(seg_trans), ptr(d_o), ptr(d_last), ptr(dq),
-            ptr(dk), ptr(dv), ptr(dg), ptr(dbeta), ptr(d_start), ptr(head_ws), ptr(seg_end), stream_of(lib, q)))
+            "pgt_gated_delta_bwd", dims, qv, kv, gv, bv, ptr(start), kept + 4 * at_e, kept + 4 * at_states if T > 16 else None,
+            kept if segs > 1 else None, ptr(d_o), ptr(d_last), ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(dbeta), ptr(d_start),
+            base + 4 * n_end if n_heads else None, base if segs > 1 else None, stream_of(lib, q)))
         return dq, dk, dv, dg, dbeta, d_start, None, None
 
 
@@ -166,9 +181,12 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, lengths=None, scale=N
             raise ValueError(f"{what}: lengths are on {lengths.device}, the inputs on {v.device}")
         if tuple(lengths.shape) not in ((B,), (B, N)):
             raise ValueError(f"{what}: lengths must be [{B}] or [{B}, {N}], got {tuple(lengths.shape)}")
-        lengths = (lengths if lengths.dim() == 2 else lengths[:, None]).clamp(0, T).to(torch.int32).expand(B, N).contiguous()
+        if lengths.dtype != torch.int32:                  # (the kernels clamp; the conversion must not wrap)
+            lengths = lengths.clamp(0, T).to(torch.int32)
+        lengths = (lengths if lengths.dim() == 2 else lengths[:, None]).expand(B, N).contiguous()
     scale = float(K) ** -0.5 if scale is None else float(scale)
-    q, k, v = _last_axis_contiguous(q), _last_axis_contiguous(k), _last_axis_contiguous(v)
+    q, k, v = _in_reach(_last_axis_contiguous(q)), _in_reach(_last_axis_contiguous(k)), _in_reach(_last_axis_contiguous(v))
+    g, beta = _in_reach(g), _in_reach(beta)
     with on_device(v):
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
                                         or initial_state is not None and initial_state.requires_grad):
