@@ -48,7 +48,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
   using TM = Team<D>;
   constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, NT = D / 16;
   constexpr int W_KQ = NW > 1 ? 1 : 0, W_OE = NW > 2 ? 2 : NW - 1, W_DG = NW > 2 ? 3 : 0;     // who does what in part 1
-  struct Lds {
+  struct alignas(16) Lds {                               // (a team whose part starts off sixteen bytes pays for every wide LDS access)
     float k[16 * LD], q[16 * LD], o[16 * LD], e[STATE ? 4 : 16 * LD], y[STATE ? 4 : 16 * LD];
     float x[STATE ? 4 : D * LD];                           // dS, for the product that contracts over its columns
     float lane4[NW == 1 ? 1 : STATE ? 2 : 5][NW == 1 ? 4 : 256];              // tiles handed from wavefront to wavefront, four values a lane

@@ -34,7 +34,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
   constexpr int NW = TM::NW, LD = TM::LD, TL = TM::TL, QD = D / 4, SB = TM::SB, TB = 16 * SB, NT = D / 16;
   constexpr bool HALF = std::is_same_v<IO, bf16>;          // keys and queries stay bf16 in LDS, products with them run on the bf16 pipe
   constexpr int LH = D + 8;                                // row stride of the bf16 tiles, in values
-  struct Lds {
+  struct alignas(16) Lds {                               // (a team whose part starts off sixteen bytes pays for every wide LDS access)
     float k[HALF ? 4 : TB * LD], q[HALF || TRANS ? 4 : TB * LD];
     uint16_t kb[HALF ? TB * LH : 8], qb[HALF && !TRANS ? TB * LH : 8];
     float inv[SB][256], p[TRANS ? 1 : SB][256];           // A operands, four values a lane
