@@ -1,0 +1,59 @@
+"""GatedDelta — a recurrent layer along time beside the GRU / LSTM cells, for every (sample, node) of a [B, T, N, C] signal.
+
+Instead of a state vector each head keeps a matrix [key, value] that is read by a query, decays, and has the difference between
+a new value and what it already holds for the key written back (the gated delta rule, ops.gated_delta_rule).  All T steps run in one
+call, forward and backward, whatever T is; a serving program advances one step at a time (`step`, ops.gated_delta_step) from the same
+state.  The heads' outputs go through a group norm with an activation, a group to a head (ops.group_norm_act), and an output product.
+There is no graph in it: put a graph convolution before or behind it, as around TemporalConv.
+"""
+import torch
+import torch.nn.functional as F
+
+from ... import ops
+from ..conv import Linear
+
+
+class GatedDelta(torch.nn.Module):
+    r"""Args: in_channels, out_channels (a multiple of heads), heads=4, key_channels=out_channels (of all heads together), activation="silu"
+    (None, "relu" or "silu", behind the norm), eps=1e-5.  Head widths (channels / heads) are at most 128."""
+
+    def __init__(self, in_channels: int, out_channels: int, heads: int = 4, key_channels: int = None, activation: str = "silu",
+                 eps: float = 1e-5):
+        super().__init__()
+        key_channels = out_channels if key_channels is None else key_channels
+        if heads < 1 or out_channels % heads or key_channels % heads:
+            raise ValueError(f"GatedDelta: {out_channels} output and {key_channels} key channels must divide over {heads} heads")
+        self.in_channels, self.out_channels, self.heads, self.key_channels = in_channels, out_channels, heads, key_channels
+        self.activation, self.eps = activation, eps
+        self.linear_qkv = Linear(in_channels, 2 * key_channels + out_channels, bias=False)
+        self.linear_gates = Linear(in_channels, 2 * heads)            # what is forgotten and what is written, per head
+        self.log_rate = torch.nn.Parameter(torch.linspace(-3.0, 0.0, heads))      # heads from slow to fast
+        self.norm_weight = torch.nn.Parameter(torch.ones(out_channels))
+        self.norm_bias = torch.nn.Parameter(torch.zeros(out_channels))
+        self.linear_out = Linear(out_channels, out_channels)
+
+    def _inputs(self, X):
+        """q, k (normalised), v, g, beta of [.., C] inputs, heads as the last axis but one."""
+        K, H = self.key_channels, self.heads
+        q, k, v = self.linear_qkv(X).split([K, K, self.out_channels], -1)
+        q, k = (F.normalize(t.unflatten(-1, (H, K // H)).float(), dim=-1).to(X.dtype) for t in (q, k))
+        forget, write = self.linear_gates(X).float().split([H, H], -1)
+        return q, k, v.unflatten(-1, (H, -1)), -self.log_rate.float().exp() * F.softplus(forget), torch.sigmoid(write)
+
+    def _output(self, o):
+        rows = o.flatten(-2).reshape(-1, self.out_channels)
+        y = ops.group_norm_act(rows, self.heads, self.norm_weight.float(), self.norm_bias.float(), self.eps, self.activation)
+        return self.linear_out(y.view(*o.shape[:-2], self.out_channels))
+
+    def initial_state(self, batch, nodes, device=None):
+        return torch.zeros(batch, nodes, self.heads, self.key_channels // self.heads, self.out_channels // self.heads, device=device)
+
+    def forward(self, X, H=None, lengths=None):
+        """X [B, T, N, in], H [B, N, heads, key, value] float32 or None, lengths [B] or [B, N] or None -> (Y [B, T, N, out], H')."""
+        o, H = ops.gated_delta_rule(*self._inputs(X), H, lengths)
+        return self._output(o), H
+
+    @torch.no_grad()
+    def step(self, X, H):
+        """One step for serving: X [B, N, in], H [B, N, heads, key, value] float32, updated in place -> Y [B, N, out]."""
+        return self._output(ops.gated_delta_step(*self._inputs(X), H))
