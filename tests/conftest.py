@@ -2,7 +2,9 @@ import glob
 import os
 import subprocess
 import sys
+import tempfile
 import warnings
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -37,10 +39,12 @@ def build_emu_library():
         return EMU_PATH
     os.makedirs(EMU_DIR, exist_ok=True)
     tmp = f"{EMU_PATH}.{os.getpid()}.tmp"       # several pytest-xdist workers may build at once: each links its own file, the
-    cmd = ["g++", "-std=c++17", "-O2", "-fPIC", "-shared", "-x", "c++", "-DPGT_EMU",       # rename is atomic, nobody maps a half-written one
-           "-I", os.path.join(ROOT, "tests", "hipemu"), "-I", os.path.join(ROOT, "include"), "-I", csrc] + srcs + \
-          ["-o", tmp]
-    subprocess.run(cmd, check=True)
+    flags = ["g++", "-std=c++17", "-O2", "-fPIC", "-x", "c++", "-DPGT_EMU",       # rename is atomic, nobody maps a half-written one
+             "-I", os.path.join(ROOT, "tests", "hipemu"), "-I", os.path.join(ROOT, "include"), "-I", csrc]
+    with tempfile.TemporaryDirectory() as objs, ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        outs = [os.path.join(objs, os.path.basename(s) + ".o") for s in srcs]           # one compiler per source, side by side
+        list(pool.map(lambda so: subprocess.run(flags + ["-c", so[0], "-o", so[1]], check=True), zip(srcs, outs)))
+        subprocess.run(["g++", "-shared", "-fPIC"] + outs + ["-o", tmp], check=True)
     os.replace(tmp, EMU_PATH)
     return EMU_PATH
 
