@@ -21,15 +21,16 @@ struct StepArgs {
 // lane.  Four wavefronts a workgroup; blockIdx.y walks the columns where a row is wider than LQ VEC.
 template <class IO, int VEC, int LQ, int NR, int WV>
 __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs a) {
-  constexpr int TEAMS = 4 / WV, RG = 64 / LQ * WV;         // states a workgroup, rows at a time
-  __shared__ float qk[TEAMS][2][128 + 4];
+  constexpr int TEAMS = 4 / WV, RG = 64 / LQ * WV, ROWS = NR * RG;         // states a workgroup, rows at a time, rows in all
+  constexpr bool DIRECT = NR <= 2;                         // few rows a lane: it reads its own k and q, past LDS
+  __shared__ float qk[TEAMS][2][DIRECT ? 4 : ROWS + 4];
   __shared__ float red[TEAMS][WV][3][LQ * VEC];
-  const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, team = wave / WV, w = wave % WV;
+  const int tid = (int)threadIdx.x, wave = tid >> 6, lane = tid & 63, team = PGT_UNIFORM(wave / WV), w = PGT_UNIFORM(wave % WV);
   const int64_t p = a.p0 + (int64_t)blockIdx.x * TEAMS + team;
   const bool live = p < a.P;
-  const int64_t pc = live ? p : 0, bn = pc / a.H;
-  const int h = (int)(pc - bn * a.H), kh = h / a.rep;
-  const int64_t b = bn / a.N, n = bn - b * a.N;
+  const int64_t pc = live ? p : 0;
+  const uint32_t bn = (uint32_t)pc / (uint32_t)a.H, b = bn / (uint32_t)a.N, n = bn - b * (uint32_t)a.N;      // (at most 2^31 states)
+  const int h = (int)((uint32_t)pc - bn * (uint32_t)a.H), kh = h / a.rep;
   const int col = (int)blockIdx.y * LQ * VEC + (lane % LQ) * VEC;      // first column of this lane
   const int row0 = w * (64 / LQ) + lane / LQ;
   float* S = a.state + pc * a.K * a.V;
@@ -49,28 +50,41 @@ __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs a) {
   const IO* vp = reinterpret_cast<const IO*>(a.v.p) + b * a.v.sb + n * a.v.sn + h * a.v.sh;
   const float g = reinterpret_cast<const float*>(a.g.p)[b * a.g.sb + n * a.g.sn + h * a.g.sh];
   const float beta = reinterpret_cast<const float*>(a.beta.p)[b * a.beta.sb + n * a.beta.sn + h * a.beta.sh];
-  for (int i = w * 64 + lane; i < 128; i += 64 * WV) {
-    qk[team][0][i] = i < a.K ? to_f32(kp[i]) : 0.f;
-    qk[team][1][i] = i < a.K ? to_f32(qp[i]) * a.scale : 0.f;
+  float kr[NR], qr[NR];
+  if (DIRECT) {
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int row = row0 + i * RG, at = row < a.K ? row : 0;
+      const float kx = to_f32(kp[at]), qx = to_f32(qp[at]);
+      kr[i] = row < a.K ? kx : 0.f;
+      qr[i] = row < a.K ? qx * a.scale : 0.f;
+    }
+  } else {
+    for (int i = w * 64 + lane; i < ROWS; i += 64 * WV) {
+      qk[team][0][i] = i < a.K ? to_f32(kp[i]) : 0.f;
+      qk[team][1][i] = i < a.K ? to_f32(qp[i]) * a.scale : 0.f;
+    }
   }
   float v[VEC];
 #pragma unroll
   for (int c = 0; c < VEC; ++c) v[c] = col + c < a.V ? to_f32(vp[col + c]) : 0.f;
   const float alpha = expf(g);
-  __syncthreads();
+  if (!DIRECT) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NR; ++i) { kr[i] = qk[team][0][row0 + i * RG]; qr[i] = qk[team][1][row0 + i * RG]; }
+  }
   float ks[VEC], qs[VEC], dot = 0.f;
 #pragma unroll
   for (int c = 0; c < VEC; ++c) ks[c] = qs[c] = 0.f;
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int row = row0 + i * RG;
-    const float kr = row < 128 ? qk[team][0][row] : 0.f, qr = row < 128 ? qk[team][1][row] : 0.f;
-    dot = fmaf(kr, qr, dot);
+    dot = fmaf(kr[i], qr[i], dot);
 #pragma unroll
     for (int c = 0; c < VEC; ++c) {
       s[i][c] *= alpha;
-      ks[c] = fmaf(kr, s[i][c], ks[c]);
-      qs[c] = fmaf(qr, s[i][c], qs[c]);
+      ks[c] = fmaf(kr[i], s[i][c], ks[c]);
+      qs[c] = fmaf(qr[i], s[i][c], qs[c]);
     }
   }
 #pragma unroll
@@ -110,9 +124,8 @@ __global__ __launch_bounds__(256) void delta_step_kernel(StepArgs a) {
   for (int i = 0; i < NR; ++i) {
     const int row = row0 + i * RG;
     if (row < a.K) {
-      const float kr = qk[team][0][row];
 #pragma unroll
-      for (int c = 0; c < VEC; ++c) s[i][c] = fmaf(kr, u[c], s[i][c]);
+      for (int c = 0; c < VEC; ++c) s[i][c] = fmaf(kr[i], u[c], s[i][c]);
       pgt_stv<VEC>(S + (int64_t)row * a.V + col, s[i]);
     }
   }

@@ -20,6 +20,10 @@ template <class IO, int VEC> __device__ __forceinline__ void get(const IO* p, fl
 #pragma unroll
   for (int c = 0; c < VEC; ++c) x[c] = to_f32(t.v[c]);
 }
+template <class IO, int VEC> __device__ __forceinline__ void open(const Pack<IO, VEC>& t, bool on, float (&x)[VEC]) {
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) x[c] = on ? to_f32(t.v[c]) : 0.f;
+}
 template <class IO, int VEC> __device__ __forceinline__ void put(IO* p, const float (&x)[VEC]) {
   Pack<IO, VEC> t;
 #pragma unroll
@@ -90,6 +94,17 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
   }
   const float inv_n = 1.f / (float)a.Cg;
   const int64_t step = (int64_t)gridDim.x * a.reps;
+  Pack<IO, VEC> nx[NV], nd[BWD ? NV : 1];                 // the next row as loaded (every load is issued, from a valid place)
+  auto fetch = [&](int64_t row) {
+    const int64_t at = (row < a.B ? row : a.B - 1) * a.C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int64_t e = at + (on[j] ? g * a.Cg + (lane + lanes * j) * VEC : 0);
+      nx[j] = *reinterpret_cast<const Pack<IO, VEC>*>(reinterpret_cast<const IO*>(a.x) + e);
+      if (BWD) nd[j] = *reinterpret_cast<const Pack<IO, VEC>*>(reinterpret_cast<const IO*>(a.dy) + e);
+    }
+  };
+  fetch((int64_t)blockIdx.x * a.reps + rep);
   for (int64_t row0 = (int64_t)blockIdx.x * a.reps; row0 < a.B; row0 += step) {
     const int64_t row = row0 + rep, at = row * a.C + (int64_t)g * a.Cg;
     const bool in = row < a.B;
@@ -97,16 +112,10 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(NormArgs a) {
     float sum = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int e = (lane + lanes * j) * VEC;
-#pragma unroll
-      for (int c = 0; c < VEC; ++c) x[j][c] = 0.f;
-      if (on[j] && in) get<IO, VEC>(reinterpret_cast<const IO*>(a.x) + at + e, x[j]);
-      if (BWD) {
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) d[j][c] = 0.f;
-        if (on[j] && in) get<IO, VEC>(reinterpret_cast<const IO*>(a.dy) + at + e, d[j]);
-      }
+      open<IO, VEC>(nx[j], on[j] && in, x[j]);
+      if (BWD) open<IO, VEC>(nd[j], on[j] && in, d[j]);
     }
+    fetch(row + step);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
@@ -219,11 +228,28 @@ template <int VEC> __device__ __forceinline__ void slice_sums(const NormArgs& a,
     }
   }
 }
-// the sums over a sample's slices of channel c
-__device__ __forceinline__ void channel_sums(const NormArgs& a, int c, float& s0, float& s1) {
+// The sums over a sample's slices of channel c, by a wavefront: `parts` (1, 2, 4, ..) runs of slices lie `width` lanes apart and are
+// added up over them, so that every lane of the wavefront reads where a group has few channels.
+__device__ __forceinline__ void channel_sums(const NormArgs& a, int c, bool in, int part, int parts, int width, float& s0, float& s1) {
   s0 = s1 = 0.f;
-  const float* p = a.ws + sample_of(a) * a.slices * 2 * a.C + c;
-  for (int i = 0; i < a.slices; ++i) { s0 += p[(int64_t)(2 * i) * a.C]; s1 += p[(int64_t)(2 * i + 1) * a.C]; }
+  const float* p = a.ws + sample_of(a) * a.slices * 2 * a.C + (in ? c : 0);
+  int i = part;
+  for (; i + 3 * parts < a.slices; i += 4 * parts) {
+    float x[4], y[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { x[u] = p[(int64_t)(2 * (i + u * parts)) * a.C]; y[u] = p[(int64_t)(2 * (i + u * parts) + 1) * a.C]; }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { s0 += x[u]; s1 += y[u]; }
+  }
+  for (; i < a.slices; i += parts) { s0 += p[(int64_t)(2 * i) * a.C]; s1 += p[(int64_t)(2 * i + 1) * a.C]; }
+  for (int m = width; m < 64; m <<= 1) { s0 += __shfl_xor(s0, m); s1 += __shfl_xor(s1, m); }
+  if (!in) s0 = s1 = 0.f;
+}
+// lanes that a group's channels take (a power of two), the runs of slices beside each other
+__device__ __forceinline__ int lanes_of_group(int Cg) {
+  int n = 1;
+  while (n < 64 && n < Cg) n <<= 1;
+  return n;
 }
 
 template <class IO, int VEC>
@@ -270,29 +296,34 @@ template <class IO> __device__ __forceinline__ void join_stats(const NormArgs& a
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
   const IO* x = reinterpret_cast<const IO*>(a.x) + sample_of(a) * a.S * a.C;
   const float inv_s = 1.f / (float)a.S;
+  const int width = lanes_of_group(a.Cg), parts = 64 / width, part = lane / width, li = lane % width;
   for (int g = g0 + wave; g < g1; g += 4) {
     float sum = 0.f, sq = 0.f, m0 = 0.f;
     const int c_lo = g * a.Cg;
-    for (int i = lane; i < a.Cg; i += 64) {
+    for (int i0 = 0; i0 < a.Cg; i0 += width) {
+      const int i = i0 + li;
+      const bool in = i < a.Cg;
       float s0, s1;
-      channel_sums(a, c_lo + i, s0, s1);
-      const float m = to_f32(x[c_lo + i]) + s0 * inv_s;
-      if (i == lane) m0 = m;
+      channel_sums(a, c_lo + i, in, part, parts, width, s0, s1);
+      const float m = in ? to_f32(x[c_lo + i]) + s0 * inv_s : 0.f;
+      if (i0 == 0) m0 = m;
       sum += m;
       sq += s1 - s0 * (s0 * inv_s);
     }
-    const float mean = gd_xsum(sum, 64) / (float)a.Cg;
+    const float mean = gd_xsum(sum, width) / (float)a.Cg;
     float dev = 0.f;
-    for (int i = lane; i < a.Cg; i += 64) {
+    for (int i0 = 0; i0 < a.Cg; i0 += width) {
+      const int i = i0 + li;
+      const bool in = i < a.Cg;
       float m = m0;
-      if (i != lane) {
+      if (i0 > 0) {
         float s0, s1;
-        channel_sums(a, c_lo + i, s0, s1);
-        m = to_f32(x[c_lo + i]) + s0 * inv_s;
+        channel_sums(a, c_lo + i, in, part, parts, width, s0, s1);
+        m = in ? to_f32(x[c_lo + i]) + s0 * inv_s : 0.f;
       }
-      dev = fmaf(m - mean, m - mean, dev);
+      if (in) dev = fmaf(m - mean, m - mean, dev);
     }
-    const float var = (gd_xsum(sq, 64) + (float)a.S * gd_xsum(dev, 64)) / ((float)a.S * (float)a.Cg);
+    const float var = (gd_xsum(sq, width) + (float)a.S * gd_xsum(dev, width)) / ((float)a.S * (float)a.Cg);
     if (lane == 0) {
       st[2 * (g - g0)] = mean;
       st[2 * (g - g0) + 1] = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
@@ -355,17 +386,20 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormArgs a) {
   if (DX) {
     const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
     const float inv_n = 1.f / ((float)a.S * (float)a.Cg);
+    const int width = lanes_of_group(a.Cg), parts = 64 / width, part = lane / width, li = lane % width;
     for (int g = g0 + wave; g < g1; g += 4) {
       float t1 = 0.f, t2 = 0.f;
-      for (int i = lane; i < a.Cg; i += 64) {
+      for (int i0 = 0; i0 < a.Cg; i0 += width) {
+        const int i = i0 + li;
+        const bool in = i < a.Cg;
         float dw, db;
-        channel_sums(a, g * a.Cg + i, dw, db);
-        const float w = a.w ? a.w[g * a.Cg + i] : 1.f;
+        channel_sums(a, g * a.Cg + i, in, part, parts, width, dw, db);
+        const float w = in && a.w ? a.w[g * a.Cg + i] : 1.f;
         t1 = fmaf(w, db, t1);
         t2 = fmaf(w, dw, t2);
       }
-      t1 = gd_xsum(t1, 64) * inv_n;
-      t2 = gd_xsum(t2, 64) * inv_n;
+      t1 = gd_xsum(t1, width) * inv_n;
+      t2 = gd_xsum(t2, width) * inv_n;
       if (lane == 0) { lds[2 * (g - g0)] = t1; lds[2 * (g - g0) + 1] = t2; }
     }
     __syncthreads();
@@ -462,7 +496,7 @@ Plan plan(int64_t B, int64_t S, int64_t C, int64_t G, int dtype, bool aligned) {
   p.vec = aligned ? widest : 1;
   while (p.vec > 1 && Cg % p.vec) p.vec >>= 1;
   const int64_t vecs = Cg / p.vec;
-  p.rows = S == 1 && vecs <= 64 * 8;
+  p.rows = S == 1 && vecs <= 64 * (p.vec == 8 ? 4 : 8);      // (more a lane does not fit the adjoint's registers)
   p.slices = p.grid_z = 1;
   p.slice_rows = S;
   if (p.rows) {
