@@ -288,6 +288,7 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
       const gd_f4 dr = mma16(take(0), du, zero4());
       PGT_SCHED_FENCE();
       gd_f4 dy, eo, ey;
+      const bool on = STATE || c > c0 || (seg == 0 && a.d_start);      // somebody asks for the gradient of this chunk's start state
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         dy[r] = beta[r] * dr[r];
@@ -295,6 +296,13 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
         eo[r] = enter[r] * dout[r];
         ey[r] = -(enter[r] * dy[r]);
       }
+      if (!STATE) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) L.x[(16 * t + 4 * cg + r) * LD + n] = S[t][r];
+      }
+      if (on)
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (t % 4 == 0) PGT_SCHED_FENCE();
@@ -303,7 +311,6 @@ __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bw
         for (int r = 0; r < 4; ++r) {
           kt[r] = L.k[(4 * cg + r) * LD + 16 * t + col];
           qt[r] = L.q[(4 * cg + r) * LD + 16 * t + col];
-          if (!STATE) L.x[(16 * t + 4 * cg + r) * LD + n] = S[t][r];
           S[t][r] *= whole;
         }
         S[t] = mma16(kt, ey, mma16(qt, eo, S[t]));

@@ -2,7 +2,6 @@
 #include "delta_common.h"
 
 #include <type_traits>
-#include <stdlib.h>
 
 using namespace gd;
 
@@ -468,14 +467,16 @@ int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s) {
   s->lengths = d->lengths;
   s->scale = d->scale;
   // Segments: a sequence is walked chunk by chunk; with few sequences most of the 256 CUs idle.  Splitting it costs two more
-  // recurrences (a segment's own addition and its transition matrix) but divides the walk.
+  // recurrences (a segment's own addition and its transition matrix) and the join, but divides the walk.  Below 512 workgroups it pays
+  // (414 sequences of 126 chunks, 32 wide: 137 us in eight segments, 163 in four, 278 in one), from there on the chip is full.  Segments
+  // are made until there are about 2048 workgroups (1400: 144 us, 2600: 144), 256 where one fills a CU (8 sequences of 512 chunks, 128
+  // wide: 32 segments 197 us, 25 214, 40 284), and no segment is shorter than four chunks.
   const int width = s->K > s->V ? s->K : s->V;
   const int64_t teams_per_wg = width <= 16 ? 4 : width <= 32 ? 2 : 1;
   const int64_t wgs = pgt_cdiv(s->P, teams_per_wg);
   int segs = 1;
-  static const int lim = getenv("GD_LIM") ? atoi(getenv("GD_LIM")) : 512, mst = getenv("GD_MOST") ? atoi(getenv("GD_MOST")) : 2048, m128 = getenv("GD_M128") ? atoi(getenv("GD_M128")) : 256;
-  if (wgs > 0 && wgs < lim && s->chunks >= 16) {
-    const int64_t most = (width > 64 ? m128 : mst) / wgs, by_length = s->chunks / 4;
+  if (wgs > 0 && wgs < 512 && s->chunks >= 16) {
+    const int64_t most = (width > 64 ? 256 : 2048) / wgs, by_length = s->chunks / 4;
     segs = (int)(most < by_length ? most : by_length);
     if (segs > 64) segs = 64;
     if (segs < 3) segs = 1;
