@@ -6,8 +6,9 @@
 //     so one pass over the data gives statistics and result, in the adjoint too (the statistics are taken again, not stored).
 //   S > 1: a sample does not fit a CU.  Two launches: sums per channel and slice of rows, then the result, every workgroup joining
 //     the slices' sums itself (they are few and in cache).  Threads keep their channels, so weights and statistics sit in registers.
-// Sums are fp32; the variance is taken from deviations from a value of the same channel (S > 1: the sample's first row) or
-// from the mean itself (S = 1), never as a difference of large squares.  No atomics: the order of every sum is fixed.
+// Sums are fp32; the variance is never a difference of large squares: S = 1 takes squares about the mean itself, S > 1 carries mean and
+// squares about it along (four rows at a time: n += 4, mean += 4 d / n, squares += their own + d^2 4 (n - 4) / n) and joins threads and
+// slices by the same rule, so that neither an offset nor a single row far off costs accuracy.  No atomics: the order of every sum is fixed.
 #include "delta_common.h"
 
 using namespace gd;
@@ -254,79 +255,131 @@ __device__ __forceinline__ int lanes_of_group(int Cg) {
 
 template <class IO, int VEC>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
-  __shared__ __attribute__((aligned(16))) float lds[256 * VEC];
+  __shared__ float lds[2][256 * VEC];
   const Place p = place<VEC>(a);
   const IO* x = reinterpret_cast<const IO*>(a.x) + sample_of(a) * a.S * a.C + p.c0;
-  float s[2][VEC], piv[VEC];
+  float mean[VEC], sq[VEC], piv[VEC], n = 0.f;            // mean: from this thread's first row, which the values are taken from first
 #pragma unroll
-  for (int c = 0; c < VEC; ++c) s[0][c] = s[1][c] = 0.f;
+  for (int c = 0; c < VEC; ++c) mean[c] = sq[c] = piv[c] = 0.f;
   if (p.on) {
-    get<IO, VEC>(x, piv);
     int64_t r = p.r0 + p.tr;
+    get<IO, VEC>(x + (r < p.r1 ? r : p.r0) * a.C, piv);
     for (; r + 3 * p.rp < p.r1; r += 4 * p.rp) {
       float v[4][VEC];
 #pragma unroll
       for (int u = 0; u < 4; ++u) get<IO, VEC>(x + (r + u * p.rp) * a.C, v[u]);
+      const float f = 4.f * gd_rcp(n + 4.f), nf = n * f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int c = 0; c < VEC; ++c) {
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) {
-          const float d = v[u][c] - piv[c];
-          s[0][c] += d;
-          s[1][c] = fmaf(d, d, s[1][c]);
-        }
+        for (int u = 0; u < 4; ++u) v[u][c] = v[u][c] - piv[c] - mean[c];
+        const float d = 0.25f * ((v[0][c] + v[1][c]) + (v[2][c] + v[3][c]));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sq[c] = fmaf(v[u][c] - d, v[u][c] - d, sq[c]);
+        sq[c] = fmaf(d * d, nf, sq[c]);
+        mean[c] = fmaf(d, f, mean[c]);
+      }
+      n += 4.f;
     }
     for (; r < p.r1; r += p.rp) {
       float v[VEC];
       get<IO, VEC>(x + r * a.C, v);
+      const float f = gd_rcp(n + 1.f), nf = n * f;
 #pragma unroll
       for (int c = 0; c < VEC; ++c) {
-        const float d = v[c] - piv[c];
-        s[0][c] += d;
-        s[1][c] = fmaf(d, d, s[1][c]);
+        const float d = v[c] - piv[c] - mean[c];
+        sq[c] = fmaf(d * d, nf, sq[c]);
+        mean[c] = fmaf(d, f, mean[c]);
       }
+      n += 1.f;
     }
   }
-  slice_sums<VEC>(a, p, s, lds);
+#pragma unroll
+  for (int c = 0; c < VEC; ++c) {
+    lds[0][(int)threadIdx.x * VEC + c] = piv[c] + mean[c];
+    lds[1][(int)threadIdx.x * VEC + c] = sq[c];
+  }
+  __syncthreads();
+  // the slice's mean and squares about it, from its threads': ws[b][slice][2][C].  Thread row r holds full + (r < rest) rows.
+  const int64_t rows = p.r1 - p.r0, full = rows / p.rp;
+  const int rest = (int)(rows - full * p.rp), have = full > 0 ? p.rp : rest;
+  for (int e = (int)threadIdx.x; e < p.nq * VEC; e += 256) {
+    const float p0 = lds[0][e];
+    float t = 0.f, q = 0.f;
+    for (int r = 0; r < have; ++r) t = fmaf((float)(full + (r < rest)), lds[0][r * p.nq * VEC + e] - p0, t);
+    const float m = p0 + t / (float)rows;
+    for (int r = 0; r < have; ++r) {
+      const float d = lds[0][r * p.nq * VEC + e] - m;
+      q += fmaf((float)(full + (r < rest)) * d, d, lds[1][r * p.nq * VEC + e]);
+    }
+    float* out = a.ws + (sample_of(a) * a.slices + blockIdx.x) * 2 * a.C + blockIdx.z * 256 * VEC + e;
+    out[0] = m;
+    out[a.C] = q;
+  }
 }
 
-// Joins the sums of a sample: per group (mean, rstd) into st[g][2].  Channel c: mean m_c = pivot + s0 / S, squares about it s1 - s0^2 / S; the
-// group's squares are those plus S (m_c - mean)^2.  Two rounds over the group's channels, a wavefront to a group.
-template <class IO> __device__ __forceinline__ void join_stats(const NormArgs& a, float* st, int g0, int g1) {
+// n values of mean m and squares q about it, joined by further ones
+struct Moments { float n, m, q; };
+__device__ __forceinline__ void join(Moments& a, float n, float m, float q) {
+  const float all = a.n + n, f = all > 0.f ? n / all : 0.f, d = m - a.m;
+  a.m = fmaf(d, f, a.m);
+  a.q += fmaf(d * d, a.n * f, q);
+  a.n = all;
+}
+// As channel_sums, for the means and squares that the slices hold.
+__device__ __forceinline__ Moments channel_moments(const NormArgs& a, int c, bool in, int part, int parts, int width) {
+  const float* p = a.ws + sample_of(a) * a.slices * 2 * a.C + (in ? c : 0);
+  const float n = (float)a.slice_rows;                    // of every slice but the last one
+  Moments t = {0.f, p[(int64_t)(2 * (part < a.slices ? part : 0)) * a.C], 0.f};
+  int i = part;
+  for (; i + 3 * parts < a.slices - 1; i += 4 * parts) {
+    float x[4], y[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { x[u] = p[(int64_t)(2 * (i + u * parts)) * a.C]; y[u] = p[(int64_t)(2 * (i + u * parts) + 1) * a.C]; }
+    float d = 0.f, q = 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { x[u] -= t.m; d = fmaf(0.25f, x[u], d); }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) q += fmaf(n * (x[u] - d), x[u] - d, y[u]);
+    join(t, 4.f * n, t.m + d, q);
+  }
+  for (; i < a.slices; i += parts)
+    join(t, i + 1 < a.slices ? n : (float)(a.S - (int64_t)i * a.slice_rows), p[(int64_t)(2 * i) * a.C], p[(int64_t)(2 * i + 1) * a.C]);
+  for (int m = width; m < 64; m <<= 1) {                  // (both sides of an exchange join the lower lanes' with the upper lanes')
+    Moments o = {__shfl_xor(t.n, m), __shfl_xor(t.m, m), __shfl_xor(t.q, m)};
+    if ((int)threadIdx.x & m) { const Moments s = o; o = t; t = s; }
+    join(t, o.n, o.m, o.q);
+  }
+  if (!in) t.m = t.q = 0.f;
+  return t;
+}
+
+// Joins a sample's slices: per group (mean, rstd) into st[g][2]; the group's squares are its channels' plus S (their mean - the group's)^2.
+// Two rounds over the group's channels, a wavefront to a group.
+__device__ __forceinline__ void join_stats(const NormArgs& a, float* st, int g0, int g1) {
   const int wave = (int)threadIdx.x >> 6, lane = (int)threadIdx.x & 63;
-  const IO* x = reinterpret_cast<const IO*>(a.x) + sample_of(a) * a.S * a.C;
-  const float inv_s = 1.f / (float)a.S;
   const int width = lanes_of_group(a.Cg), parts = 64 / width, part = lane / width, li = lane % width;
   for (int g = g0 + wave; g < g1; g += 4) {
     float sum = 0.f, sq = 0.f, m0 = 0.f;
     const int c_lo = g * a.Cg;
     for (int i0 = 0; i0 < a.Cg; i0 += width) {
       const int i = i0 + li;
-      const bool in = i < a.Cg;
-      float s0, s1;
-      channel_sums(a, c_lo + i, in, part, parts, width, s0, s1);
-      const float m = in ? to_f32(x[c_lo + i]) + s0 * inv_s : 0.f;
-      if (i0 == 0) m0 = m;
-      sum += m;
-      sq += s1 - s0 * (s0 * inv_s);
+      const Moments t = channel_moments(a, c_lo + i, i < a.Cg, part, parts, width);
+      if (i0 == 0) m0 = t.m;
+      sum += t.m;
+      sq += t.q;
     }
     const float mean = gd_xsum(sum, width) / (float)a.Cg;
     float dev = 0.f;
     for (int i0 = 0; i0 < a.Cg; i0 += width) {
       const int i = i0 + li;
-      const bool in = i < a.Cg;
-      float m = m0;
-      if (i0 > 0) {
-        float s0, s1;
-        channel_sums(a, c_lo + i, in, part, parts, width, s0, s1);
-        m = in ? to_f32(x[c_lo + i]) + s0 * inv_s : 0.f;
-      }
-      if (in) dev = fmaf(m - mean, m - mean, dev);
+      const float m = i0 == 0 ? m0 : channel_moments(a, c_lo + i, i < a.Cg, part, parts, width).m;
+      if (i < a.Cg) dev = fmaf(m - mean, m - mean, dev);
     }
     const float var = (gd_xsum(sq, width) + (float)a.S * gd_xsum(dev, width)) / ((float)a.S * (float)a.Cg);
     if (lane == 0) {
       st[2 * (g - g0)] = mean;
-      st[2 * (g - g0) + 1] = 1.f / sqrtf((var < 0.f ? 0.f : var) + a.eps);
+      st[2 * (g - g0) + 1] = 1.f / sqrtf(var + a.eps);
     }
   }
 }
@@ -337,7 +390,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
   const Place p = place<VEC>(a);
   const int clo = (int)blockIdx.z * 256 * VEC, chi = clo + p.nq * VEC;
   const int g0 = clo / a.Cg, g1 = (chi - 1) / a.Cg + 1;
-  join_stats<IO>(a, st, g0, g1);
+  join_stats(a, st, g0, g1);
   __syncthreads();
   if (a.stats && blockIdx.x == 0)
     for (int i = (int)threadIdx.x; i < 2 * (g1 - g0); i += 256) a.stats[(sample_of(a) * a.G + g0) * 2 + i] = st[i];

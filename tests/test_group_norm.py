@@ -88,6 +88,22 @@ def test_far_means_keep_the_variance(backend):
         assert error(y, formula(x.to(F64), 4, None, None, None)) <= 2.0 ** -14
 
 
+@pytest.mark.parametrize("far", [60.0, 1e4])
+@pytest.mark.parametrize("row", [0, 1234])
+def test_a_row_far_off_keeps_the_variance(backend, far, row):
+    """A single row `far` widths off, the sample's first one among them: the variance's terms are sums of squares about means that have
+    this row in them, none a difference, so the bound of the other cases holds (four rows a thread, 128 threads and eight slices a sum)."""
+    x, w, b, dy = make((2, 4000, 8), torch.float32, 17)
+    x[:, row] += far
+    leaves = [t.to(F64).requires_grad_() for t in (x, w, b)]
+    y = formula(leaves[0], 2, leaves[1], leaves[2], None)
+    dev = [t.to(backend.device).requires_grad_() for t in (x, w, b)]
+    got = ops.group_norm_act(dev[0], 2, dev[1], dev[2])
+    assert error(got, y) <= FP32
+    for a, want in zip(torch.autograd.grad(got, dev, dy.to(backend.device)), torch.autograd.grad(y, leaves, dy.to(F64))):
+        assert error(a, want) <= 2 * FP32
+
+
 def test_only_some_gradients(backend):
     x, w, b, dy = make((3, 5, 8), torch.float32, 1)
     for shape in ((3, 5, 8), (15, 8)):
