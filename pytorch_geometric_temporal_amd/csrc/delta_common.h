@@ -82,20 +82,6 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ bf16 from_f32<bf16>(float x) { return bf16{gd_to_bf16(x)}; }
 template <> __device__ __forceinline__ f16 from_f32<f16>(float x) { return f16{gd_to_f16(x)}; }
 
-// four values of a row from p on, of which the first n exist (the others are 0); vec: p is aligned to four values and n is 4 or <= 0
-__device__ __forceinline__ gd_f4 load4(const float* p, int n, bool vec) {
-  gd_f4 r;
-  r[0] = r[1] = r[2] = r[3] = 0.f;
-  if (vec) {
-    if (n >= 4) { const float4 t = *reinterpret_cast<const float4*>(p); r[0] = t.x; r[1] = t.y; r[2] = t.z; r[3] = t.w; }
-    return r;
-  }
-  if (n > 0) r[0] = p[0];
-  if (n > 1) r[1] = p[1];
-  if (n > 2) r[2] = p[2];
-  if (n > 3) r[3] = p[3];
-  return r;
-}
 __device__ __forceinline__ gd_f4 zero4() { gd_f4 r; r[0] = r[1] = r[2] = r[3] = 0.f; return r; }
 __device__ __forceinline__ gd_f4 lds4(const float* p) {
   const float4 t = *reinterpret_cast<const float4*>(p);

@@ -4,7 +4,7 @@ Instead of a state vector each head keeps a matrix [key, value] that is read by 
 a new value and what it already holds for the key written back (the gated delta rule, ops.gated_delta_rule).  All T steps run in one
 call, forward and backward, whatever T is; a serving program advances one step at a time (`step`, ops.gated_delta_step) from the same
 state.  The heads' outputs go through a group norm with an activation, a group to a head (ops.group_norm_act), and an output product.
-There is no graph in it: put a graph convolution before or behind it, as around TemporalConv.
+The layer is float32, as its products are.  There is no graph in it: put a graph convolution before or behind it, as around TemporalConv.
 """
 import torch
 import torch.nn.functional as F
@@ -46,7 +46,10 @@ class GatedDelta(torch.nn.Module):
         return self.linear_out(y.view(*o.shape[:-2], self.out_channels))
 
     def initial_state(self, batch, nodes, device=None):
-        return torch.zeros(batch, nodes, self.heads, self.key_channels // self.heads, self.out_channels // self.heads, device=device)
+        """Zeros [batch, nodes, heads, key, value], on the layer's device unless another is given."""
+        device = self.norm_weight.device if device is None else device
+        return torch.zeros(batch, nodes, self.heads, self.key_channels // self.heads, self.out_channels // self.heads, dtype=torch.float32,
+                           device=device)
 
     def forward(self, X, H=None, lengths=None):
         """X [B, T, N, in], H [B, N, heads, key, value] float32 or None, lengths [B] or [B, N] or None -> (Y [B, T, N, out], H')."""

@@ -163,7 +163,8 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, lengths=None, scale=N
     read in place as long as the last axis is contiguous).  q and k are used as they are: normalise them before.
     initial_state [B, N, H, K, V] float32 or None (zeros).  lengths: int32 / int64 [B] or [B, N] on the same device, how many steps of each
     sequence there are: the steps behind are not looked at, their outputs and gradients are 0 (values outside 0 .. T are clamped).
-    scale: default K ** -0.5.  g = -inf forgets the state.
+    scale: default K ** -0.5.  g = -inf forgets the state.  A sample's step (N * H * V and N * Hk * K values; N * H * K where a
+    gradient is asked for) has to stay below 2^25 values, B * N * H below 2^31; other sizes are refused.
 
     Returns (o [B, T, N, H, V] in v's type, final_state [B, N, H, K, V] float32), both differentiable (once).  Products and states are
     held in float32 whatever the inputs' type; results and gradients are bitwise reproducible."""
@@ -190,6 +191,8 @@ def gated_delta_rule(q, k, v, g, beta, initial_state=None, lengths=None, scale=N
     with on_device(v):
         if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad or beta.requires_grad
                                         or initial_state is not None and initial_state.requires_grad):
+            if N * H * K >= (1 << 25) - 128:              # (what the adjoint would refuse after the forward pass has run)
+                raise ValueError(f"{what}: {N} nodes x {H} heads x {K} key columns are too many for a gradient (2^25 values a step)")
             return GatedDeltaFunction.apply(q, k, v, g, beta, initial_state, lengths, scale)
         return _forward(q, k, v, g, beta, initial_state, lengths, scale, False)[:2]
 
@@ -217,4 +220,5 @@ def gated_delta_step(q, k, v, g, beta, state, scale=None):
         else:
             _timed("gated_delta_step", 8.0 * state.numel(), lambda: lib.call(
                 "pgt_gated_delta_step", dims, *views, state.data_ptr(), o.data_ptr(), stream_of(lib, v)))
+    torch.autograd.graph.increment_version(state)         # a graph that kept the state must not read the new one as the old
     return o

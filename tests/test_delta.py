@@ -126,6 +126,18 @@ def test_long_sequences_run_in_segments(backend, case, ragged):
     check_rule(backend, d, r, case, torch.float32, torch.tensor([T - 150]) if ragged else None)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("case", [(1, 272, 1, 1, 2, 16, 16), (2, 300, 1, 1, 1, 32, 32), (1, 275, 1, 1, 2, 64, 64), (2, 280, 1, 1, 1, 128, 128)],
+                         ids=lambda c: "x".join(map(str, c)))
+def test_segments_at_whole_widths(backend, case, dtype):
+    """Every whole width and type in segments, one sequence of two ending before the last segments where there are two."""
+    B, T, N, Hk, H, K, V = case
+    d, r = inputs(*case, dtype, seed=T + 1)
+    dims = _lib.DeltaDimsStruct(B, T, N, Hk, H, K, V, TYPES.index(dtype), 1.0, None)
+    assert _lib.get_lib()._pgt_gated_delta_segments(dims) > 2
+    check_rule(backend, d, r, case, dtype, torch.tensor([70, T]) if B == 2 else None)
+
+
 def test_lengths_of_zero_and_one_and_outside(backend):
     case = (5, 20, 2, 1, 1, 6, 5)
     d, r = inputs(*case, torch.float32, seed=4)
@@ -286,6 +298,17 @@ def test_steps_continue_a_sequence(backend):
     assert error(state, S.cpu().to(F64)) <= tolerance(12, 8, 20)
 
 
+def test_a_step_on_a_state_that_a_graph_kept_is_noticed(backend):
+    d, r = inputs(1, 3, 2, 1, 2, 8, 4, torch.float32, seed=3)
+    d = {n: x.to(backend.device) for n, x in d.items()}
+    k = d["k"].requires_grad_()
+    _, last = ops.gated_delta_rule(d["q"], k, d["v"], d["g"], d["beta"], d["start"])
+    with torch.no_grad():
+        ops.gated_delta_step(d["q"][:, 0], k[:, 0], d["v"][:, 0], d["g"][:, 0], d["beta"][:, 0], d["start"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        last.sum().backward()
+
+
 def test_refusals(backend):
     d, _ = inputs(1, 4, 2, 1, 2, 6, 5, torch.float32)
     good = {n: x.to(backend.device) for n, x in d.items()}
@@ -316,6 +339,14 @@ def test_refusals(backend):
     with pytest.raises(RuntimeError, match="no gradient"):
         ops.gated_delta_step(*(one[n].clone().requires_grad_() for n in names), state)
     assert torch.equal(state, good["start"])
+
+
+def test_a_gradient_too_wide_is_refused_before_the_forward_pass(backend):
+    N = 1 << 18
+    z = lambda *s: torch.zeros(1, device=backend.device).expand(*s)  # noqa: E731
+    q, v, gate = z(1, 1, N, 1, 128), z(1, 1, N, 1, 1), z(1, 1, N, 1)
+    with pytest.raises(ValueError, match="too many for a gradient"):
+        ops.gated_delta_rule(q, q, v, gate, gate.detach().requires_grad_())
 
 
 def test_bad_arguments_at_the_c_entries_return_codes(backend):
