@@ -43,6 +43,8 @@ struct BwdArgs {
 // product itself read down columns.  Bound by the fp32 matrix pipe from K = 64 on (2 K + 22 MFMAs of 32 cycles a wavefront and chunk).
 // STATE: only the gradient of the state before the segment, from a zero gradient behind it (the last segment: from d_last).
 // VEC: every row can be read four values at a time; FULL: K = V = D besides.
+// Measured: 52 992 sequences of 12 steps, 16 x 16, fp32: 137 us (2.2 TB/s; vector instructions busy half of the time, MFMA 28 %).  1656 sequences
+// of 288 steps, 32 x 32, fp32: 250 us (828 workgroups, three a CU: the last round is nearly empty).
 template <class IO, int D, bool STATE, bool FULL, bool VEC>
 __global__ __launch_bounds__(Team<D>::THREADS, Team<D>::WAVES_BWD) void delta_bwd_kernel(BwdArgs a) {
   using TM = Team<D>;

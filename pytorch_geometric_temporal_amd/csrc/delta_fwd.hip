@@ -27,6 +27,9 @@ struct FwdArgs {
 // TRANS: what a long sequence with few heads is split with: blockIdx.z 0: only the state behind the segment, from a zero start (the
 // first segment: from the sequence's); 1: the segment's transition matrix, i.e. the same recurrence with v = 0 from the unit matrix.
 // VEC: rows can be read four values at a time; FULL: K = V = D besides.
+// Measured: 52 992 sequences of 12 steps, 16 x 16, fp32: 58 us = 3.8 TB/s.  414 sequences of 2016 steps, 32 x 32, bf16, in eight segments:
+// TRANS 70 us, join 13, main 66.  8 sequences of 8191 steps, 128 x 128, bf16, in 32 segments: TRANS 80 us, join 74, main 57 (each chunk
+// about 3.5 us, a chain of products that nothing but another segment can overlap).
 template <class IO, int D, bool TRANS, bool FULL, bool VEC>
 __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void delta_fwd_kernel(FwdArgs a) {
   using TM = Team<D>;

@@ -1,7 +1,8 @@
 // Gated delta rule, one step of every sequence, the state updated in place (delta_common.h has the rule):
 //   held = exp(g) S^T k,  u = beta (v - held),  S <- exp(g) S + k u^T,  o = scale S^T q = scale (exp(g) S_old^T q + (q . k) u).
 // The second form of o takes both products from ONE pass over the old state, which then waits in registers for its update: the
-// state crosses HBM once each way and nothing else is of size.  Bound by that traffic (8 K V bytes a sequence).
+// state crosses HBM once each way and nothing else is of size.  Bound by that traffic (8 K V bytes a sequence): 400 000 states of 16 x 16 in
+// 195 us = 4.7 TB/s, 4096 of 128 x 128 (bf16 inputs) in 108 us = 5.0 TB/s; 828 states of 16 x 16 take 3.7 us, a launch.
 #include "delta_common.h"
 
 using namespace gd;
