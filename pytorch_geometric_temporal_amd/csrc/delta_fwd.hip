@@ -20,6 +20,11 @@ struct FwdArgs {
   int vec;                       // q, k, v rows can be read four values at a time
 };
 
+// where the join finds element (row, column) of a transition matrix [D, D]: [row / 16][column / 16][lane][4]
+template <int D> __device__ __forceinline__ int trans_at(int row, int column) {
+  return ((row / 16 * (D / 16) + column / 16) * 64 + column % 16 / 4 * 16 + row % 16) * 4 + column % 4;
+}
+
 // One team per sequence and segment of chunks; a wavefront owns sixteen columns of the state.  Blocks of SB chunks: the tiles that do
 // not depend on the state (P, the inverse, the decays) are prepared first, one chunk a wavefront side by side, then every wavefront walks
 // the block's chunks alone, without a barrier.  A chunk's walk is 3 K / 4 + 8 v_mfma_f32_16x16x4_f32 of 32 cycles, the fp32 matrix
@@ -28,7 +33,7 @@ struct FwdArgs {
 // first segment: from the sequence's); 1: the segment's transition matrix, i.e. the same recurrence with v = 0 from the unit matrix.
 // VEC: rows can be read four values at a time; FULL: K = V = D besides.
 // Measured: 52 992 sequences of 12 steps, 16 x 16, fp32: 58 us = 3.8 TB/s.  414 sequences of 2016 steps, 32 x 32, bf16, in eight segments:
-// TRANS 70 us, join 13, main 66.  8 sequences of 8191 steps, 128 x 128, bf16, in 32 segments: TRANS 80 us, join 74, main 57 (each chunk
+// TRANS 70 us, join 13, main 66.  8 sequences of 8191 steps, 128 x 128, bf16, in 32 segments: TRANS 83 us, join 54, main 57 (each chunk
 // about 3.5 us, a chain of products that nothing but another segment can overlap).
 template <class IO, int D, bool TRANS, bool FULL, bool VEC>
 __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void delta_fwd_kernel(FwdArgs a) {
@@ -334,7 +339,20 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
     if (unit) { to = a.seg_trans + (sq.p * (s.segs - 2) + seg - 1) * K * K; ld = K; }
     else if (TRANS) to = a.seg_start + (sq.p * (s.segs - 1) + seg) * K * V;
     else to = seg == s.segs - 1 ? a.last + sq.p * K * V : nullptr;
-    if (to) store_state<NT, FULL>(S, to, K, ld, n, cg);
+    if (unit && to && (FULL || K == D)) {                 // in the join's tiles, turned in LDS (all of it is free behind the last block)
+      static_assert(sizeof(Lds) >= NW * 320 * sizeof(float), "a tile a wavefront");
+      float* turn = reinterpret_cast<float*>(&L) + w * 320;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        gd_wave_sync();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) turn[(4 * cg + r) * 20 + col] = S[t][r];
+        gd_wave_sync();
+        put4(to + ((t * NT + w) * 64 + lane) * 4, lds4(&turn[col * 20 + 4 * cg]));
+      }
+    } else if (to) {
+      store_state<NT, FULL>(S, to, K, ld, n, cg);
+    }
     if (!TRANS) {                                         // rows behind the sequence: zero
       const int lo = 16 * (ce > c0 ? ce : c0), hi = 16 * c1 < s.T ? 16 * c1 : s.T;
       for (int t = lo + tok; t < hi; t += 16) {
@@ -350,7 +368,9 @@ __global__ __launch_bounds__(Team<D>::THREADS, TRANS ? 4 : Team<D>::WAVES) void 
 // x [P, segs - 1, K, V] holds the second summand and takes the sum (its entry 0 is complete already).  UP (the adjoint): from the last
 // entry down with the transposed transitions.  A workgroup owns sixteen columns of a sequence's state, a wavefront sixteen rows; the
 // next two transitions are on their way while one is multiplied: what remains of a step is its K / 4 dependent MFMAs and one barrier.
-template <int D, bool UP, bool VEC, bool FULL>
+// Transitions of whole width (K = D) lie in 16 x 16 tiles as the product's left operand takes them, a kilobyte in a row a load (TILED): read
+// row by row, sixteen rows a load, 31 joins of 8 states of 128 x 128 took 74 us, 54 in tiles.
+template <int D, bool UP, bool TILED, bool VEC, bool FULL>
 __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* trans, float* x, int segs, int K_, int V_) {
   const int K = FULL ? D : K_, V = FULL ? D : V_;       // FULL: every lane stores, and the compiler knows how much is in flight
   constexpr int LD = D + 4, NT = D / 16;
@@ -362,8 +382,9 @@ __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* 
   float* x0 = x + p * entries * K * V;
   float* xp = x0 + (int64_t)row0 * V + n;
   const float* mp = trans + p * (segs - 2) * K * K;
-  const int at_m = UP ? 4 * cg * K + i : i * K + 4 * cg;
-  gd_f4 m0[NT], m1[NT], add0, add1;
+  const int at_m = TILED ? (UP ? trans_at<D>(4 * cg, i) : trans_at<D>(i, 4 * cg)) : UP ? 4 * cg * K + i : i * K + 4 * cg;
+  constexpr int AHEAD = TILED && !UP ? 4 : 2;                      // transitions on their way
+  gd_f4 m[AHEAD][NT], add[AHEAD];
   auto fetch = [&](int j, gd_f4 (&m)[NT], gd_f4& add) {                               // step j: entry `to` takes the transition of segment `tr`
     const int to = UP ? entries - 1 - j : j, tr = UP ? entries - j : j;
     const float* q = mp + (int64_t)(tr - 1) * K * K;
@@ -371,7 +392,12 @@ __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* 
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int left = i < K ? K - 16 * t - 4 * cg : 0;
-      if (VEC) {
+      if (TILED && !UP) {
+        m[t] = lds4(q + at_m + 256 * t);
+      } else if (TILED) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m[t][r] = q[at_m + 256 * NT * t + 4 * r];
+      } else if (VEC) {
         m[t] = lds4(q + (left > 0 ? at_m + 16 * t : 0));
       } else {
 #pragma unroll
@@ -394,19 +420,21 @@ __global__ __launch_bounds__(64 * (D / 16)) void delta_join_kernel(const float* 
 #pragma unroll
     for (int t = 0; t < NT; ++t) s = mma16(m[t], lds4(&buf[col * LD + 16 * t + 4 * cg]), s);
     const int to = UP ? entries - 1 - j : j;
-    fetch(j + 2 < entries ? j + 2 : entries - 1, m, add);  // (always: with a branch here every step would wait for all loads)
+    fetch(j + AHEAD < entries ? j + AHEAD : entries - 1, m, add);  // (always: with a branch here every step would wait for all loads)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (FULL || (row0 + r < K && n < V)) xp[((int64_t)to * K + r) * V] = s[r];
   };
-  fetch(1, m0, add0);
-  fetch(entries > 2 ? 2 : 1, m1, add1);
+#pragma unroll
+  for (int u = 0; u < AHEAD; ++u) fetch(1 + u < entries ? 1 + u : entries - 1, m[u], add[u]);
   int j = 1;
-  for (; j + 1 < entries; j += 2) {
-    step(j, m0, add0);
-    step(j + 1, m1, add1);
+  for (; j + AHEAD - 1 < entries; j += AHEAD) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) step(j + u, m[u], add[u]);
   }
-  if (j < entries) step(j, m0, add0);
+#pragma unroll
+  for (int u = 0; u < AHEAD - 1; ++u)
+    if (j + u < entries) step(j + u, m[u], add[u]);
 }
 
 template <class IO, int D, bool TRANS, bool FULL, bool VEC> void go(const FwdArgs& a0, pgt_stream_t stream) {
@@ -422,9 +450,10 @@ template <class IO, int D, bool TRANS, bool FULL, bool VEC> void go(const FwdArg
 }
 template <int D, bool UP> void join(const float* trans, float* x, int64_t P, int segs, int K, int V, pgt_stream_t stream) {
   const dim3 grid((unsigned)P, (unsigned)((V + 15) / 16)), block(64 * (D / 16));
-  if (K == D && V == D && pgt_aligned(trans, 16)) PGT_LAUNCH((delta_join_kernel<D, UP, !UP, true>), grid, block, stream, trans, x, segs, K, V);
-  else if (!UP && K % 4 == 0 && pgt_aligned(trans, 16)) PGT_LAUNCH((delta_join_kernel<D, UP, !UP, false>), grid, block, stream, trans, x, segs, K, V);
-  else PGT_LAUNCH((delta_join_kernel<D, UP, false, false>), grid, block, stream, trans, x, segs, K, V);
+  if (K == D && V == D) PGT_LAUNCH((delta_join_kernel<D, UP, true, false, true>), grid, block, stream, trans, x, segs, K, V);
+  else if (K == D) PGT_LAUNCH((delta_join_kernel<D, UP, true, false, false>), grid, block, stream, trans, x, segs, K, V);
+  else if (!UP && K % 4 == 0) PGT_LAUNCH((delta_join_kernel<D, UP, false, !UP, false>), grid, block, stream, trans, x, segs, K, V);
+  else PGT_LAUNCH((delta_join_kernel<D, UP, false, false, false>), grid, block, stream, trans, x, segs, K, V);
 }
 template <class IO, int D> void all(const FwdArgs& a, pgt_stream_t stream) {
   const bool full = a.vec && a.s.K == D && a.s.V == D;
@@ -473,7 +502,7 @@ int pgt_delta_shape(const pgt_delta_dims* d, const char* who, gd::Shape* s) {
   // recurrences (a segment's own addition and its transition matrix) and the join, but divides the walk.  Below 512 workgroups it pays
   // (414 sequences of 126 chunks, 32 wide: 137 us in eight segments, 163 in four, 278 in one), from there on the chip is full.  Segments
   // are made until there are about 2048 workgroups (1400: 144 us, 2600: 144), 256 where one fills a CU (8 sequences of 512 chunks, 128
-  // wide: 32 segments 197 us, 25 214, 40 284), and no segment is shorter than four chunks.
+  // wide: 32 segments 197 us, 25 214, 40 284; 179 since the joins read tiles), and no segment is shorter than four chunks.
   const int width = s->K > s->V ? s->K : s->V;
   const int64_t teams_per_wg = width <= 16 ? 4 : width <= 32 ? 2 : 1;
   const int64_t wgs = pgt_cdiv(s->P, teams_per_wg);
@@ -527,6 +556,7 @@ extern "C" int pgt_gated_delta_fwd(const pgt_delta_dims* d, const pgt_seq_view* 
     a.vec = 0;
   }
   PGT_REQUIRE(a.s.segs == 1 || (seg_start && seg_trans), "pgt_gated_delta_fwd: a sequence in %d segments needs seg_start and seg_trans", a.s.segs);
+  PGT_REQUIRE(a.s.segs == 1 || pgt_aligned(seg_trans, 16), "pgt_gated_delta_fwd: seg_trans must be aligned to 16 bytes");
   a.start = start; a.o = o; a.last = last; a.e = e; a.states = states; a.seg_start = seg_start; a.seg_trans = seg_trans;
   if (d->dtype == PGT_DT_F32) by_width<float>(a, stream);
   else if (d->dtype == PGT_DT_BF16) by_width<bf16>(a, stream);

@@ -127,10 +127,11 @@ def test_long_sequences_run_in_segments(backend, case, ragged):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
-@pytest.mark.parametrize("case", [(1, 272, 1, 1, 2, 16, 16), (2, 300, 1, 1, 1, 32, 32), (1, 275, 1, 1, 2, 64, 64), (2, 280, 1, 1, 1, 128, 128)],
+@pytest.mark.parametrize("case", [(1, 272, 1, 1, 2, 16, 16), (2, 300, 1, 1, 1, 32, 32), (1, 275, 1, 1, 2, 64, 64), (1, 257, 1, 1, 1, 128, 128),
+                                  (1, 272, 1, 1, 1, 16, 9), (1, 257, 1, 1, 1, 64, 48)],
                          ids=lambda c: "x".join(map(str, c)))
 def test_segments_at_whole_widths(backend, case, dtype):
-    """Every whole width and type in segments, one sequence of two ending before the last segments where there are two."""
+    """Every whole key width and type in segments, with value widths equal and smaller, one sequence of two ending before the last segments where there are two."""
     B, T, N, Hk, H, K, V = case
     d, r = inputs(*case, dtype, seed=T + 1)
     dims = _lib.DeltaDimsStruct(B, T, N, Hk, H, K, V, TYPES.index(dtype), 1.0, None)
